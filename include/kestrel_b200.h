@@ -50,7 +50,8 @@ enum {
   KB200_DTYPE_F32 = 0,
   KB200_DTYPE_F16 = 1,
   KB200_DTYPE_BF16 = 2,
-  KB200_DTYPE_E4M3 = 3 /* FP8 e4m3fn codes, one byte per element */
+  KB200_DTYPE_E4M3 = 3, /* FP8 e4m3fn codes, one byte per element */
+  KB200_DTYPE_I8 = 4    /* int8 codes with one fp32 scale per block (a page of one KV head): (code + 1/2) * scale */
 };
 
 /* Bits of device status word 0 (kb200_device_status). */
@@ -60,7 +61,10 @@ enum {
   KB200_STATUS_BAD_ROW = 4,     /* a page-table row index outside the table (row skipped) */
   KB200_STATUS_WAIT_TIMEOUT = 8, /* a bounded wait on a shared-memory barrier ran out */
   KB200_STATUS_BAD_POSITION = 16, /* rotary: a position outside the cos/sin table (clamped) */
-  KB200_STATUS_BAD_PREFIX = 32   /* attention: shared_prefix_pages covers keys a query row may not see */
+  KB200_STATUS_BAD_PREFIX = 32,  /* attention: shared_prefix_pages covers keys a query row may not see */
+  KB200_STATUS_NOT_FINITE = 64,  /* int8 append: a row holds NaN (stored as code 0) or an infinity (saturated) */
+  KB200_STATUS_NO_PAGES = 128    /* ragged step: it does not fit the free list or the token buffers (nothing taken);
+                                    release: more pages than the free list holds (nothing released) */
 };
 
 KB200_API int kb200_abi_version(void);
@@ -269,6 +273,13 @@ typedef struct kb200_attn_args {
    * the batch.  A sequence that breaks the promise sets KB200_STATUS_BAD_PREFIX. */
   int32_t shared_prefix_pages;
   int32_t reserved0;
+
+  /* Scales of int8 pools (kv_dtype == KB200_DTYPE_I8, else ignored): device fp32 [n_pages, H_kv] with unit head stride,
+   * one non-negative scale per page and KV head; an element is (code + 1/2) * scale.  k_scale, v_scale and the
+   * per-head vectors do not apply.  A caller built without these fields passes its own, smaller struct_bytes. */
+  const float* k_block_scale;
+  const float* v_block_scale;
+  int64_t block_scale_page_stride;
 } kb200_attn_args;
 
 /* Scratch bytes kb200_paged_attention needs for the given problem bounds. */
@@ -319,6 +330,106 @@ KB200_API int kb200_sample_step_from_logits(
     const void* logits, int32_t logits_dtype, int64_t batch, int64_t vocab, int64_t row_stride,
     const float* temperatures, const float* top_ps, const float* uniforms, int64_t* out_ids,
     float* logprobs, int32_t device, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Append to int8 pools with one scale per block, a block being one page of one KV head.
+ * (No reference counterpart: its 8-bit pools are e4m3 with a scale per layer, kestrel/kv_cache.py:159-172.)
+ *
+ * scale: the power of two s with 64 s <= max|x| < 128 s over the block's rows (0 for a block of zeros, at least
+ * 2^-126 otherwise); code = floor(x / s), so an element is (code + 1/2) s within s / 2.  A block whose first token
+ * (slot % page_size == 0) is written starts anew; otherwise its scale never falls, and when it grows by 2^k
+ * the codes the block holds become code >> k.  The bytes of a block therefore do not depend on how its tokens were
+ * split over calls.
+ *
+ *   key, value        as kb200_reshape_and_cache_flash (F32 / F16 / BF16), head_dim a multiple of 16
+ *   key_cache, value_cache   device int8 cache views, 16-byte aligned, strides multiples of 16
+ *   key_scales, value_scales  device fp32 [n_pages, n_kv_heads], page stride given in elements
+ *   slot_mapping      device int64 [num_tokens]; negative slots are skipped.  The tokens of one block are
+ *                     neighbours in the mapping, as any layout by sequence leaves them; a block whose tokens come in
+ *                     two separate runs of one call is left with undefined codes (nothing else is touched).  Of
+ *                     equal slots in a run the last one counts.
+ */
+KB200_API int kb200_append_block_int8(
+    const void* key, const void* value, int64_t key_token_stride, int64_t value_token_stride, void* key_cache,
+    void* value_cache, int64_t cache_page_stride, int64_t cache_token_stride, int64_t cache_head_stride,
+    float* key_scales, float* value_scales, int64_t scale_page_stride, const int64_t* slot_mapping,
+    int64_t num_tokens, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int32_t in_dtype,
+    int32_t device, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The tables of one ragged step, built on the GPU from request lengths in one launch: pages taken from a free list
+ * in device memory (the order of PageTable.reserve called entry after entry, kestrel/kv_cache.py:366-407), block
+ * table, slot mapping, positions and packed row offsets for any mix of decode rows and prompt chunks.
+ *
+ *   page_table     device int32 [pt_rows, pt_cols]: the requests' rows; new entries are written
+ *   batch_idx      device int32 / int64 [batch]: row of each entry.  Distinct, but for row 0, the padding row: it is
+ *                  never given pages (its entries map to whatever row 0 holds, page 0 as a rule)
+ *   lengths        device int32 [batch]: tokens each entry holds; new_tokens int32 [batch]: tokens it appends
+ *   free_pages     device int32 [free_capacity], the first *free_count of them free; pages leave from the end
+ *   out_page_table device int32 [batch, out_cols]: the entries' rows up to their last token, the tail untouched
+ *   out_seqused_k  int32 [batch] = lengths + new_tokens (may be `lengths`); out_cu_seqlens_q int32 [batch + 1]
+ *   out_slots, out_positions   int64 [n_tokens], packed; -1 and 0 behind the last token
+ *   out_free_count int32 [1] (may be `free_count`); out_pages_taken int32 [1]
+ * All or nothing: a step that needs more pages than are free, or more tokens than n_tokens, takes nothing
+ * (out_pages_taken = -1, no tokens, out_seqused_k = lengths) and sets KB200_STATUS_NO_PAGES.  An entry with a row
+ * outside the table, a negative count or more tokens than a row holds gets no tokens, out_seqused_k = 0 and
+ * KB200_STATUS_BAD_ROW.  batch <= 8192.
+ */
+KB200_API int kb200_build_ragged_step(
+    int32_t* page_table, int64_t pt_row_stride, int64_t pt_rows, int64_t pt_cols, const void* batch_idx,
+    int32_t batch_idx_is_i64, const int32_t* lengths, const int32_t* new_tokens, const int32_t* free_pages,
+    int64_t free_capacity, const int32_t* free_count, int32_t* out_page_table, int64_t out_row_stride,
+    int64_t out_cols, int32_t* out_seqused_k, int32_t* out_cu_seqlens_q, int64_t* out_slots, int64_t* out_positions,
+    int64_t n_tokens, int32_t* out_free_count, int32_t* out_pages_taken, int64_t batch, int64_t n_pages,
+    int32_t page_size, int32_t device, void* stream);
+
+/* Gives the pages of finished requests back to the free list, last page of a row first (PageTable.erase,
+ * kestrel/kv_cache.py:430-446).  keep_pages int32 [batch] or NULL: leading pages of each row that stay allocated.
+ * The released table entries become -1; *free_count grows. */
+KB200_API int kb200_release_rows(
+    int32_t* page_table, int64_t pt_row_stride, int64_t pt_rows, int64_t pt_cols, const void* batch_idx,
+    int32_t batch_idx_is_i64, const int32_t* lengths, const int32_t* keep_pages, int32_t* free_pages,
+    int64_t free_capacity, int32_t* free_count, int64_t batch, int32_t page_size, int32_t device, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search, selection: the n_out best continuations of each request over beams and vocabulary,
+ * cand(w, v) = score_w + logit_wv - logsumexp_v(logit_w), largest first, equal ones by the lowest w * vocab + v.
+ *
+ *   logits     device [batch * beams, vocab] of F32 / F16 / BF16, row stride given; a NaN counts as -inf
+ *   scores     device fp32 [batch, beams], finite or -inf (anything else counts as -inf)
+ *   finished   device uint8 [batch, beams] or NULL: such a beam has one continuation, end_token, at its own score
+ *   out_tokens, out_parents int64, out_scores fp32: [batch, n_out]; the parent is the beam inside the request
+ * Rows without a finite log-sum-exp have only candidates of -inf.  beams <= 64, n_out <= 64, vocab <= 2^20.
+ */
+KB200_API uint64_t kb200_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n_out, int32_t device);
+KB200_API int kb200_beam_step_from_logits(
+    const void* logits, int32_t logits_dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,
+    const float* scores, const uint8_t* finished, int64_t end_token, int64_t n_out, int64_t* out_tokens,
+    int64_t* out_parents, float* out_scores, void* workspace, uint64_t workspace_bytes, int32_t device, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search, reordering: beam w of request b goes on from beam parents[b, w].
+ * Every beam has private pages (`own_table`); `beam_table` is what attention reads: full pages may be another beam's,
+ * the page being filled is always the beam's own.  With L = lengths[b] tokens in each beam of the request, the table
+ * entries of the L / P full pages are gathered and, when L mod P > 0, the first L mod P tokens of the parent's
+ * private page L / P are copied to the beam's own (in every pool), with the blocks' scales.  In place, in any
+ * permutation and with repeats.
+ *
+ *   pools      HOST array of device base pointers: the K and V pools of every layer, [n_pages, n_heads, page_size,
+ *              row] with row_bytes bytes per token and head; strides in bytes
+ *   scales     HOST array (n_scales, may be 0) of device fp32 [n_pages, n_heads] scale arrays of int8 pools
+ *   beam_table device int32 [batch * beams, table_cols]; own_table device int32 [own_n_rows, own_cols]
+ *   own_rows   device int64 [batch * beams] or NULL: row of own_table of each beam (NULL: its own number)
+ *   parents    device int32 / int64 [batch, beams], each in [0, beams); others leave the beam as it is (BAD_ROW)
+ * beams <= 32.
+ */
+KB200_API int kb200_reorder_beam_pages(
+    void* const* pools, int32_t n_pools, float* const* scales, int32_t n_scales, int64_t page_stride_bytes,
+    int64_t head_stride_bytes, int32_t row_bytes, int32_t n_heads, int64_t scale_page_stride, int64_t n_pages,
+    int32_t* beam_table, int64_t table_row_stride, int64_t table_cols, const int32_t* own_table,
+    int64_t own_row_stride, int64_t own_n_rows, int64_t own_cols, const int64_t* own_rows, const void* parents,
+    int32_t parents_is_i64, const int32_t* lengths, int64_t batch, int32_t beams, int32_t page_size, int32_t device,
+    void* stream);
 
 /* ---------------------------------------------------------------------------
  * kb200_paged_attention without a caller-provided scratch buffer.  This entry

@@ -13,10 +13,11 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libkestrel_b200.so"
 ABI_VERSION = 4
 
-DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2, 3
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_I8 = 0, 1, 2, 3, 4
 STATIC_SCRATCH_BYTES = 32 * 1024 * 1024  # KB200_STATIC_SCRATCH_BYTES
 
 STATUS_BAD_SLOT, STATUS_BAD_PAGE, STATUS_BAD_ROW, STATUS_WAIT_TIMEOUT, STATUS_BAD_POSITION, STATUS_BAD_PREFIX = 1, 2, 4, 8, 16, 32
+STATUS_NOT_FINITE, STATUS_NO_PAGES = 64, 128
 
 # Every symbol include/kestrel_b200.h declares.
 EXPORTS = (
@@ -35,6 +36,12 @@ EXPORTS = (
     "kb200_block_visibility",
     "kb200_paged_attention_static",
     "kb200_sample_step_from_logits",
+    "kb200_append_block_int8",
+    "kb200_build_ragged_step",
+    "kb200_release_rows",
+    "kb200_beam_workspace_bytes",
+    "kb200_beam_step_from_logits",
+    "kb200_reorder_beam_pages",
 )
 
 
@@ -91,6 +98,9 @@ class AttnArgs(C.Structure):
         ("q_visible_batch_stride", C.c_int64),
         ("shared_prefix_pages", C.c_int32),
         ("reserved0", C.c_int32),
+        ("k_block_scale", C.c_void_p),
+        ("v_block_scale", C.c_void_p),
+        ("block_scale_page_stride", C.c_int64),
     ]
 
 
@@ -140,6 +150,27 @@ def _declare(lib: C.CDLL) -> None:
     lib.kb200_paged_attention.argtypes = [C.POINTER(AttnArgs)]
     lib.kb200_sample_step_from_logits.restype = C.c_int
     lib.kb200_sample_step_from_logits.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp, vp, vp, i32, vp]
+    lib.kb200_append_block_int8.restype = C.c_int
+    lib.kb200_append_block_int8.argtypes = [
+        vp, vp, i64, i64, vp, vp, i64, i64, i64, vp, vp, i64, vp, i64, i64, i32, i32, i32, i32, i32, vp,
+    ]
+    lib.kb200_build_ragged_step.restype = C.c_int
+    lib.kb200_build_ragged_step.argtypes = [
+        vp, i64, i64, i64, vp, i32, vp, vp, vp, i64, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp, vp, i64, i64, i32, i32, vp,
+    ]
+    lib.kb200_release_rows.restype = C.c_int
+    lib.kb200_release_rows.argtypes = [vp, i64, i64, i64, vp, i32, vp, vp, vp, i64, vp, i64, i32, i32, vp]
+    lib.kb200_beam_workspace_bytes.restype = C.c_uint64
+    lib.kb200_beam_workspace_bytes.argtypes = [i64, i64, i64, i64, i32]
+    lib.kb200_beam_step_from_logits.restype = C.c_int
+    lib.kb200_beam_step_from_logits.argtypes = [
+        vp, i32, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, C.c_uint64, i32, vp,
+    ]
+    lib.kb200_reorder_beam_pages.restype = C.c_int
+    lib.kb200_reorder_beam_pages.argtypes = [
+        C.POINTER(vp), i32, C.POINTER(vp), i32, i64, i64, i32, i32, i64, i64, vp, i64, i64, vp, i64, i64, i64, vp, vp, i32, vp,
+        i64, i32, i32, i32, vp,
+    ]
     lib.kb200_paged_attention_static.restype = C.c_int
     lib.kb200_paged_attention_static.argtypes = [C.POINTER(AttnArgs)]
 

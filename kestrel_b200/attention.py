@@ -26,7 +26,7 @@ def paged_attention(query: torch.Tensor, *, paged_kv_layer: Any, page_table: tor
     """``query [B, H_q, S, D]`` against one paged K/V layer; returns ``[B, S, H_q, D]`` in the query dtype.
 
     ``paged_kv_layer``: ``k_cache`` / ``v_cache`` ``[n_pages, H_kv, P, D]`` and, for FP8 pools, ``k_scale`` /
-    ``v_scale``.  ``paged_kv_seqlens_k`` counts each sequence's keys including the tokens just appended.
+    ``v_scale``, for int8 pools ``k_block_scale`` / ``v_block_scale`` (one scale per page and KV head).  ``paged_kv_seqlens_k`` counts each sequence's keys including the tokens just appended.
     Mask: causal, bottom-right aligned; with ``sliding_window = W`` each query sees the last ``W`` keys up to
     its own position.  ``paged_kv_seqlens_q`` limits the valid query rows per sequence (padded layout);
     with ``cu_seqlens_q`` the ``B * S`` rows are handed over packed instead.
@@ -49,6 +49,8 @@ def paged_attention(query: torch.Tensor, *, paged_kv_layer: Any, page_table: tor
         cu_seqlens_q=cu_seqlens_q, max_seqlen_q=n_rows if packed else None,
         paged_kv_non_tma=True, softmax_scale=scaling,
         k_scale=getattr(paged_kv_layer, "k_scale", None), v_scale=getattr(paged_kv_layer, "v_scale", None),
+        k_block_scale=getattr(paged_kv_layer, "k_block_scale", None),
+        v_block_scale=getattr(paged_kv_layer, "v_block_scale", None),
         shared_prefix_pages=shared_prefix_pages, **mask)
     return out.view(n_seq, n_rows, n_heads, head_dim) if packed else out
 

@@ -52,6 +52,7 @@ inline int dtype_size(int dt) {
     case KB200_DTYPE_F16: return 2;
     case KB200_DTYPE_BF16: return 2;
     case KB200_DTYPE_E4M3: return 1;
+    case KB200_DTYPE_I8: return 1;
     default: return 0;
   }
 }
@@ -142,6 +143,9 @@ enum KernelId : int {
   KID_ROPE_APPEND = 8,
   KID_PREFILL = 9,
   KID_SAMPLE = 10,
+  KID_APPEND_I8 = 11,
+  KID_RAGGED = 12,
+  KID_REORDER = 13,
 };
 
 }  // namespace kb200

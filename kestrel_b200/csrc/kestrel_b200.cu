@@ -6,6 +6,9 @@
 #include "paged_attention.cuh"
 #include "paged_prefill.cuh"
 #include "sampling.cuh"
+#include "block_int8.cuh"
+#include "ragged_step.cuh"
+#include "beam.cuh"
 
 using namespace kb200;
 
@@ -133,8 +136,10 @@ uint64_t kb200_attn_workspace_bytes(int64_t batch, int64_t total_q, int32_t n_q_
   return need;
 }
 
-uint64_t kb200_attn_workspace_bytes_for(const kb200_attn_args* args) {
-  if (!args || args->struct_bytes != sizeof(kb200_attn_args)) return 0;
+uint64_t kb200_attn_workspace_bytes_for(const kb200_attn_args* given) {
+  kb200_attn_args full;
+  if (!given || !attn_args_in_full(given, &full)) return 0;
+  const kb200_attn_args* args = &full;
   if (args->batch <= 0 || args->total_q <= 0 || args->n_q_heads <= 0 || args->n_kv_heads <= 0 || args->head_dim <= 0)
     return 0;
   int sms = 0;
@@ -160,8 +165,91 @@ int kb200_sample_step_from_logits(const void* logits, int32_t logits_dtype, int6
 
 int kb200_paged_attention(const kb200_attn_args* args) {
   if (!args) return fail(KB200_ERR_INVALID, "args is null");
-  KB200_ENTER(args->device);
-  return launch_paged_attention(args);
+  kb200_attn_args full;
+  if (!attn_args_in_full(args, &full))
+    return fail(KB200_ERR_INVALID, "kb200_attn_args size mismatch: got %u, built with %zu", args->struct_bytes, sizeof(full));
+  KB200_ENTER(full.device);
+  return launch_paged_attention(&full);
+}
+
+int kb200_append_block_int8(const void* key, const void* value, int64_t key_token_stride, int64_t value_token_stride,
+                            void* key_cache, void* value_cache, int64_t cache_page_stride, int64_t cache_token_stride,
+                            int64_t cache_head_stride, float* key_scales, float* value_scales, int64_t scale_page_stride,
+                            const int64_t* slot_mapping, int64_t num_tokens, int64_t n_pages, int32_t page_size,
+                            int32_t n_kv_heads, int32_t head_dim, int32_t in_dtype, int32_t device, void* stream) {
+  KB200_ENTER(device);
+  return launch_append_block_int8(key, value, key_token_stride, value_token_stride, key_cache, value_cache,
+                                  cache_page_stride, cache_token_stride, cache_head_stride, key_scales, value_scales,
+                                  scale_page_stride, slot_mapping, num_tokens, n_pages, page_size, n_kv_heads, head_dim,
+                                  in_dtype, static_cast<cudaStream_t>(stream));
+}
+
+int kb200_build_ragged_step(int32_t* page_table, int64_t pt_row_stride, int64_t pt_rows, int64_t pt_cols,
+                            const void* batch_idx, int32_t batch_idx_is_i64, const int32_t* lengths,
+                            const int32_t* new_tokens, const int32_t* free_pages, int64_t free_capacity,
+                            const int32_t* free_count, int32_t* out_page_table, int64_t out_row_stride, int64_t out_cols,
+                            int32_t* out_seqused_k, int32_t* out_cu_seqlens_q, int64_t* out_slots, int64_t* out_positions,
+                            int64_t n_tokens, int32_t* out_free_count, int32_t* out_pages_taken, int64_t batch,
+                            int64_t n_pages, int32_t page_size, int32_t device, void* stream) {
+  KB200_ENTER(device);
+  KB200_REQUIRE(batch <= 0x7fffffff, "batch out of range");
+  RaggedParams p;
+  p.page_table = page_table; p.pt_rs = pt_row_stride; p.pt_rows = pt_rows; p.pt_cols = pt_cols;
+  p.batch_idx = batch_idx; p.batch_idx_is_i64 = batch_idx_is_i64;
+  p.lengths = lengths; p.new_tokens = new_tokens;
+  p.free_pages = free_pages; p.free_cap = free_capacity; p.free_count = free_count;
+  p.out_page_table = out_page_table; p.out_rs = out_row_stride; p.out_cols = out_cols;
+  p.out_seqused = out_seqused_k; p.out_cu = out_cu_seqlens_q;
+  p.out_slots = out_slots; p.out_positions = out_positions; p.n_tokens = n_tokens;
+  p.out_free_count = out_free_count; p.out_taken = out_pages_taken;
+  p.batch = (int)batch; p.n_pages = n_pages; p.page_size = page_size;
+  return launch_ragged_step(p, device, static_cast<cudaStream_t>(stream));
+}
+
+int kb200_release_rows(int32_t* page_table, int64_t pt_row_stride, int64_t pt_rows, int64_t pt_cols, const void* batch_idx,
+                       int32_t batch_idx_is_i64, const int32_t* lengths, const int32_t* keep_pages, int32_t* free_pages,
+                       int64_t free_capacity, int32_t* free_count, int64_t batch, int32_t page_size, int32_t device,
+                       void* stream) {
+  KB200_ENTER(device);
+  KB200_REQUIRE(batch <= 0x7fffffff, "batch out of range");
+  ReleaseParams p;
+  p.page_table = page_table; p.pt_rs = pt_row_stride; p.pt_rows = pt_rows; p.pt_cols = pt_cols;
+  p.batch_idx = batch_idx; p.batch_idx_is_i64 = batch_idx_is_i64;
+  p.lengths = lengths; p.keep = keep_pages;
+  p.free_pages = free_pages; p.free_cap = free_capacity; p.free_count = free_count;
+  p.batch = (int)batch; p.page_size = page_size;
+  return launch_release_rows(p, device, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t kb200_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n_out, int32_t device) {
+  if (batch <= 0 || beams <= 0 || vocab <= 0 || n_out <= 0) return 0;
+  int sms = 0;
+  if (device_sm_count(device, &sms) != KB200_OK) return 0;
+  return beam_workspace_need(batch, beams, vocab, n_out, sms);
+}
+
+int kb200_beam_step_from_logits(const void* logits, int32_t logits_dtype, int64_t batch, int64_t beams, int64_t vocab,
+                                int64_t row_stride, const float* scores, const uint8_t* finished, int64_t end_token,
+                                int64_t n_out, int64_t* out_tokens, int64_t* out_parents, float* out_scores,
+                                void* workspace, uint64_t workspace_bytes, int32_t device, void* stream) {
+  KB200_ENTER(device);
+  return launch_beam_step(logits, logits_dtype, batch, beams, vocab, row_stride, scores, finished, end_token, n_out,
+                          out_tokens, out_parents, out_scores, workspace, workspace_bytes, device,
+                          static_cast<cudaStream_t>(stream));
+}
+
+int kb200_reorder_beam_pages(void* const* pools, int32_t n_pools, float* const* scales, int32_t n_scales,
+                             int64_t page_stride_bytes, int64_t head_stride_bytes, int32_t row_bytes, int32_t n_heads,
+                             int64_t scale_page_stride, int64_t n_pages, int32_t* beam_table, int64_t table_row_stride,
+                             int64_t table_cols, const int32_t* own_table, int64_t own_row_stride, int64_t own_n_rows,
+                             int64_t own_cols, const int64_t* own_rows, const void* parents, int32_t parents_is_i64,
+                             const int32_t* lengths, int64_t batch, int32_t beams, int32_t page_size, int32_t device,
+                             void* stream) {
+  KB200_ENTER(device);
+  return launch_reorder(pools, n_pools, scales, n_scales, page_stride_bytes, head_stride_bytes, row_bytes, n_heads,
+                        scale_page_stride, n_pages, beam_table, table_row_stride, table_cols, own_table, own_row_stride,
+                        own_n_rows, own_cols, own_rows, parents, parents_is_i64, lengths, batch, beams, page_size, device,
+                        static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
@@ -198,11 +286,13 @@ int static_scratch_address(int device, void** out) {
 
 extern "C" {
 
-int kb200_paged_attention_static(const kb200_attn_args* args) {
-  if (!args) return fail(KB200_ERR_INVALID, "args is null");
-  if (args->struct_bytes != sizeof(kb200_attn_args))
-    return fail(KB200_ERR_INVALID, "kb200_attn_args size mismatch: got %u, built with %zu", args->struct_bytes,
+int kb200_paged_attention_static(const kb200_attn_args* given) {
+  if (!given) return fail(KB200_ERR_INVALID, "args is null");
+  kb200_attn_args full;
+  if (!attn_args_in_full(given, &full))
+    return fail(KB200_ERR_INVALID, "kb200_attn_args size mismatch: got %u, built with %zu", given->struct_bytes,
                 sizeof(kb200_attn_args));
+  const kb200_attn_args* args = &full;
   KB200_ENTER(args->device);
   if (args->batch > 0 && args->total_q > 0) {
     const uint64_t need = kb200_attn_workspace_bytes_for(args);

@@ -128,6 +128,10 @@ struct AttnParams {
   const char* k_base;
   const char* v_base;
   long long kv_ps_b, kv_ts_b, kv_hs_b;
+  // int8 pools: scale of (page, KV head), [n_pages, H_kv] with the given page stride
+  const float* kbs;
+  const float* vbs;
+  long long bs_ps;
 };
 
 // Where the attention kernels read the plan from: shared memory (built by the CTA itself) or the
@@ -274,6 +278,41 @@ __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t x, uint32_t& lo, uint32
       : "=r"(lo), "=r"(hi)
       : "r"(x));
 }
+// Four int8 codes (one 32-bit word) -> code + 1/2 as f16, bytes 0 and 2 in `lo`, bytes 1 and 3 in `hi`; exact.  In
+// [512, 1024) an f16 has steps of 1/2: the code's eight bits, its sign flipped, go to mantissa bits 1-8 and a one to bit 0,
+// which makes 512 + (code + 128) + 1/2.
+__device__ __forceinline__ void i8x4_to_f16x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = ((x << 1) & 0x01fe01feu) ^ 0x61016101u, b = ((x >> 7) & 0x01fe01feu) ^ 0x61016101u;
+  const __half2 c = __float2half2_rn(640.f);
+  const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&a), c), rb = __hsub2(*reinterpret_cast<const __half2*>(&b), c);
+  lo = *reinterpret_cast<const uint32_t*>(&ra);
+  hi = *reinterpret_cast<const uint32_t*>(&rb);
+}
+// the pairs that i8x4_to_f16x4 makes, for four consecutive 16-bit elements in two words
+__device__ __forceinline__ void pair_02_13(uint32_t& w0, uint32_t& w1) {
+  const uint32_t e = __byte_perm(w0, w1, 0x5410), o = __byte_perm(w0, w1, 0x7632);
+  w0 = e;
+  w1 = o;
+}
+// int8 pools: what a warp has to know of a tile besides its codes, the scales of its keys (lane l: keys l and l + 32)
+template <int KPL>
+struct TileScales {
+  float k[KPL], v[KPL];
+  // of key base + off of the tile; base: a constant of an unrolled loop, off < 8
+  __device__ __forceinline__ float key(int base, int off) const { return __shfl_sync(0xffffffffu, k[base >> 5], (base & 31) + off); }
+  __device__ __forceinline__ float val(int base, int off) const { return __shfl_sync(0xffffffffu, v[base >> 5], (base & 31) + off); }
+  __device__ __forceinline__ float max_val() const {   // (scales are not negative: ordered as integers)
+    uint32_t m = __float_as_uint(v[0]);
+#pragma unroll
+    for (int u = 1; u < KPL; ++u) m = max(m, __float_as_uint(v[u]));
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+  }
+};
+// The weights of an int8 tile carry the keys' V scales, relative to the largest scale seen (V and P are f16 operands):
+// 2^15 / 2^8 of headroom keep small blocks next to large ones in f16's normal range.
+constexpr float kVScaleUp = 32768.f;       // weights of at most 1
+constexpr float kVScaleUpLazy = 128.f;     // weights of at most 2^8 (lazily raised maximum)
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF16) {
@@ -601,13 +640,29 @@ struct TileProducer {
     advance_after_issue();
   }
   __device__ __forceinline__ bool more() const { return issued < my_tiles; }
+  // int8 pools: the scales of the tile that the next issue() fetches.  Keys past the end of the sequence get 0.
+  template <int KPL>
+  __device__ __forceinline__ void fetch_scales(TileScales<KPL>& ts) const {
+    const int k0 = (pc.tile0 + pc.t) * TILE_N;
+#pragma unroll
+    for (int u = 0; u < KPL; ++u) {
+      const int i = lane + 32 * u, key = k0 + i;
+      int page;
+      if constexpr (GATHER) page = key < pc.L ? pt_row[key >> p_shift] : -1;
+      else page = __shfl_sync(0xffffffffu, pg, (i >> box_shift) << 1);   // (rows of at most 128 bytes: K and V, a box each)
+      const bool ok = key < pc.L && (unsigned)page < (unsigned long long)p.n_pages;
+      ts.k[u] = ok ? p.kbs[page * p.bs_ps + h] : 0.f;
+      ts.v[u] = ok ? p.vbs[page * p.bs_ps + h] : 0.f;
+    }
+  }
 };
 
 // ---------------------------------------------------------------------------
 // The attention kernel.  KVB: bytes per K/V element (2: bf16/f16, 1: e4m3);
 // BF16: operand type of the MMAs (bf16 when K/V are bf16, else f16).
+// I8: K/V are int8 codes with a scale per (page, head): scores are multiplied by the key's K scale, weights by its V scale.
 // ---------------------------------------------------------------------------
-template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER>
+template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER, bool I8 = false>
 __global__ void __launch_bounds__(NW * 32, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ AttnParams p) {
@@ -658,12 +713,21 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   TileProducer<T, KVB, GATHER> prod(p, plan, &tmK, &tmV, my_stage0, bar0, lane, r0, my_tiles);
   Cursor cc = prod.pc;   // consumer side: starts where the producer starts
   if (lane == 0 && w > 0) write_boundary_record(p, w, cc);
-  for (int s = 0; s < NS && prod.more(); ++s) prod.issue(s);
+  [[maybe_unused]] TileScales<(TILE_N + 31) / 32> sc_cur, sc_next;   // (I8) scales of the tile being read and of the next one
+  if constexpr (I8) {
+    static_assert(KVB == 1 && NS == 2, "two tiles' scales are kept");
+    prod.fetch_scales(sc_cur);
+    prod.issue(0);
+    if (prod.more()) { prod.fetch_scales(sc_next); prod.issue(1); }
+  } else {
+    for (int s = 0; s < NS && prod.more(); ++s) prod.issue(s);
+  }
 
   uint32_t qf[NQF][4];
   float o[NOT][4];
   float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
   float sl2 = 0.f, vscale = 1.f;
+  [[maybe_unused]] float vref = 0.f, vinv = 0.f;   // (I8) largest V scale seen, and what a V scale is multiplied by
   int lim0 = 0, lim1 = 0, row0 = 0, row1 = 0, h = 0;
   bool valid0 = false, valid1 = false;
   bool fresh = true;
@@ -687,6 +751,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       lim1 = upper ? cc.L - cc.sq + j1 : cc.L - 1;
       const float ksc = p.ks_vec ? p.ks_vec[h] : p.ks;
       vscale = p.vs_vec ? p.vs_vec[h] : p.vs;
+      if constexpr (I8) { vref = vinv = 0.f; }
       sl2 = p.softmax_scale * ksc * kLog2e;
       m0 = m1 = -INFINITY;
       l0 = l1 = 0.f;
@@ -721,6 +786,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             b.x = pack2<false>(bf16_bits_to_float(b.x & 0xffffu), bf16_bits_to_float(b.x >> 16));
             b.y = pack2<false>(bf16_bits_to_float(b.y & 0xffffu), bf16_bits_to_float(b.y >> 16));
           }
+          if constexpr (I8) { pair_02_13(a.x, a.y); pair_02_13(b.x, b.y); }
           qf[ch][0] = a.x; qf[ch][1] = b.x; qf[ch][2] = a.y; qf[ch][3] = b.y;
         }
       }
@@ -778,10 +844,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t b0, b1;
-            e4m3x4_to_f16x4(x[i], b0, b1);
+            if constexpr (I8) i8x4_to_f16x4(x[i], b0, b1);
+            else e4m3x4_to_f16x4(x[i], b0, b1);
             mma16816<false>(s[n], qf[q4 * 4 + i], b0, b1);
           }
         }
+      }
+    }
+
+    if constexpr (I8) {
+#pragma unroll
+      for (int n = 0; n < NT8; ++n) {
+        const float ka = sc_cur.key(n * 8, 2 * c4), kb = sc_cur.key(n * 8, 2 * c4 + 1);
+        s[n][0] *= ka; s[n][1] *= kb; s[n][2] *= ka; s[n][3] *= kb;
       }
     }
 
@@ -826,6 +901,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       m0 = mn0;
       m1 = mn1;
     }
+    if constexpr (I8) {
+      const float vmax = sc_cur.max_val();
+      if (vmax > vref) {   // (warp-uniform) O is kept in units of the largest V scale
+        const float f = vref / vmax;
+#pragma unroll
+        for (int i = 0; i < NOT; ++i) {
+          o[i][0] *= f; o[i][1] *= f; o[i][2] *= f; o[i][3] *= f;
+        }
+        vref = vmax;
+        vinv = kVScaleUp / vmax;
+        vscale = vmax * (1.f / kVScaleUp);
+      }
+    }
     const float ms0 = (m0 == -INFINITY) ? 0.f : m0 * sl2;
     const float ms1 = (m1 == -INFINITY) ? 0.f : m1 * sl2;
     uint32_t pf[NKS][4];
@@ -837,8 +925,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const float p3 = ex2(fmaf(s[n][3], sl2, -ms1));
       l0 += p0 + p1;
       l1 += p2 + p3;
-      pf[n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0, p1);
-      pf[n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2, p3);
+      if constexpr (I8) {
+        const float va = sc_cur.val(n * 8, 2 * c4) * vinv, vb = sc_cur.val(n * 8, 2 * c4 + 1) * vinv;
+        pf[n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0 * va, p1 * vb);
+        pf[n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2 * va, p3 * vb);
+      } else {
+        pf[n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0, p1);
+        pf[n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2, p3);
+      }
     }
 
     // ---- O += P V.  Rows of V past the sequence end may hold anything (NaN
@@ -876,30 +970,39 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             ldsm_x4_t(x0, x1, x2, x3, addr);
             if constexpr (MASKED) { x0 &= mk_lo; x1 &= mk_hi; x2 &= mk_lo; x3 &= mk_hi; }
             // word = [key 2c: d, d+1 | key 2c+1: d, d+1]  ->  [d: key 2c, 2c+1 | d+1: key 2c, 2c+1]
-            x0 = __byte_perm(x0, 0, 0x3120);
-            x1 = __byte_perm(x1, 0, 0x3120);
-            x2 = __byte_perm(x2, 0, 0x3120);
-            x3 = __byte_perm(x3, 0, 0x3120);
+            if constexpr (!I8) {   // (the int8 conversion pairs bytes 0, 2 and 1, 3 as it is)
+              x0 = __byte_perm(x0, 0, 0x3120);
+              x1 = __byte_perm(x1, 0, 0x3120);
+              x2 = __byte_perm(x2, 0, 0x3120);
+              x3 = __byte_perm(x3, 0, 0x3120);
+            }
+            auto widen = [](uint32_t x, uint32_t& e, uint32_t& o_) {
+              if constexpr (I8) i8x4_to_f16x4(x, e, o_);
+              else e4m3x4_to_f16x4(x, e, o_);
+            };
             uint32_t e0, o0, e1, o1;
-            e4m3x4_to_f16x4(x0, e0, o0);
-            e4m3x4_to_f16x4(x1, e1, o1);
+            widen(x0, e0, o0);
+            widen(x1, e1, o1);
             mma16816<false>(o[4 * q2 + 0], pf[ks], e0, e1);  // d = 16*(2*q2)   + 2g
             mma16816<false>(o[4 * q2 + 1], pf[ks], o0, o1);  // d = 16*(2*q2)   + 2g + 1
-            e4m3x4_to_f16x4(x2, e0, o0);
-            e4m3x4_to_f16x4(x3, e1, o1);
+            widen(x2, e0, o0);
+            widen(x3, e1, o1);
             mma16816<false>(o[4 * q2 + 2], pf[ks], e0, e1);  // d = 16*(2*q2+1) + 2g
             mma16816<false>(o[4 * q2 + 3], pf[ks], o0, o1);  // d = 16*(2*q2+1) + 2g + 1
           }
         }
       }
     };
-    if (key0 + TILE_N > cc.L) pv(std::true_type{});
+    // (int8 codes are numbers whatever they are, and the weights of keys past the end are zero)
+    if (!I8 && key0 + TILE_N > cc.L) pv(std::true_type{});
     else pv(std::false_type{});
 
     // ---- this stage has been read: refill it with the tile NS ahead
     __syncwarp();
+    if constexpr (I8) sc_cur = sc_next;
     if (prod.more()) {
       fence_proxy_async();
+      if constexpr (I8) prod.fetch_scales(sc_next);
       prod.issue(stage);
     }
 
@@ -956,6 +1059,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const int64_t slot = (int64_t)seg_id + w;
         float* po = p.part_o + slot * (kRowsPerSeg * HD);
         float* pml = p.part_ml + slot * (kRowsPerSeg * 2);
+        if constexpr (I8) {   // (the merge multiplies by a scale that is 1 for such pools)
+#pragma unroll
+          for (int i = 0; i < NOT; ++i) {
+            o[i][0] *= vscale; o[i][1] *= vscale; o[i][2] *= vscale; o[i][3] *= vscale;
+          }
+        }
         if (c4 == 0) {
           if (valid0) *reinterpret_cast<float2*>(pml + g8 * 2) = make_float2((m0 == -INFINITY) ? -INFINITY : m0 * sl2, l0);
           if (valid1) *reinterpret_cast<float2*>(pml + (g8 + 8) * 2) = make_float2((m1 == -INFINITY) ? -INFINITY : m1 * sl2, l1);
@@ -1028,7 +1137,7 @@ __device__ __forceinline__ void mma16816r(float (&d)[4], uint32_t a0, uint32_t a
   }
 }
 
-template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER>
+template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER, bool I8 = false>
 __global__ void __launch_bounds__(NW * 32, 1)
 paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const __grid_constant__ AttnParams p) {
@@ -1086,7 +1195,15 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   TileProducer<T, KVB, GATHER> prod(p, plan, &tmK, &tmV, my_stage0, bar0, lane, r0, my_tiles);
   Cursor cc = prod.pc;   // consumer side: starts where the producer starts
   if (lane == 0 && w > 0) write_boundary_record(p, w, cc);
-  for (int s = 0; s < NS && prod.more(); ++s) prod.issue(s);
+  [[maybe_unused]] TileScales<(TILE_N + 31) / 32> sc_cur, sc_next;   // (I8) scales of the tile being read and of the next one
+  if constexpr (I8) {
+    static_assert(KVB == 1 && NS == 2, "two tiles' scales are kept");
+    prod.fetch_scales(sc_cur);
+    prod.issue(0);
+    if (prod.more()) { prod.fetch_scales(sc_next); prod.issue(1); }
+  } else {
+    for (int s = 0; s < NS && prod.more(); ++s) prod.issue(s);
+  }
 
   // lane-constant parts of the ldmatrix addresses
   const int mi = lane >> 3;                                  // which of the four 8x8 matrices this lane addresses
@@ -1099,6 +1216,7 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   float o[NDT][4];       // O^T: [d slice][ (d row g, q 2c) (d row g, q 2c+1) (d row g+8, q 2c) (d row g+8, q 2c+1) ]
   float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;   // running max / partial sum of query rows 2c and 2c+1
   float sl2 = 0.f, vscale = 1.f;
+  [[maybe_unused]] float vref = 0.f, vinv = 0.f;   // (I8) largest V scale seen, and what a V scale is multiplied by
   int lim0 = 0, lim1 = 0, h = 0, mb = 0;
   bool fresh = true;
   long long piece_start = r0;
@@ -1117,6 +1235,7 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       lim1 = upper ? cc.L - cc.sq + q1 / p.group : cc.L - 1;
       const float ksc = p.ks_vec ? p.ks_vec[h] : p.ks;
       vscale = p.vs_vec ? p.vs_vec[h] : p.vs;
+      if constexpr (I8) { vref = vinv = 0.f; }
       sl2 = p.softmax_scale * ksc * kLog2e;
       m0 = m1 = -INFINITY;
       l0 = l1 = 0.f;
@@ -1155,6 +1274,7 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             a.x = pack2<false>(bf16_bits_to_float(a.x & 0xffffu), bf16_bits_to_float(a.x >> 16));
             a.y = pack2<false>(bf16_bits_to_float(a.y & 0xffffu), bf16_bits_to_float(a.y >> 16));
           }
+          if constexpr (I8) pair_02_13(a.x, a.y);
           qb[ch][0] = a.x;
           qb[ch][1] = a.y;
         }
@@ -1181,6 +1301,10 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     const uint32_t vbase = kbase + T::KV_TILE_BYTES;
     const int key0 = (cc.tile0 + cc.t) * TILE_N;
 
+    auto widen = [](uint32_t x, uint32_t& e, uint32_t& o_) {
+      if constexpr (I8) i8x4_to_f16x4(x, e, o_);
+      else e4m3x4_to_f16x4(x, e, o_);
+    };
     // ---- S^T = K Q^T.  Two accumulator sets (even / odd d slices) keep dependent MMAs apart.
     float s[NMT][4], s2[NMT][4];
 #pragma unroll
@@ -1214,11 +1338,11 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           uint32_t x0, x1, x2, x3;  // (keys lo, ch) (keys hi, ch) (keys lo, ch+1) (keys hi, ch+1)
           ldsm_x4(x0, x1, x2, x3, addr);
           uint32_t a0, a1, a2, a3;
-          e4m3x4_to_f16x4(x0, a0, a2);
-          e4m3x4_to_f16x4(x1, a1, a3);
+          widen(x0, a0, a2);
+          widen(x1, a1, a3);
           mma16816r<false>(s[mt], a0, a1, a2, a3, qb[2 * cp][0], qb[2 * cp][1]);
-          e4m3x4_to_f16x4(x2, a0, a2);
-          e4m3x4_to_f16x4(x3, a1, a3);
+          widen(x2, a0, a2);
+          widen(x3, a1, a3);
           mma16816r<false>(s2[mt], a0, a1, a2, a3, qb[2 * cp + 1][0], qb[2 * cp + 1][1]);
         }
       }
@@ -1228,6 +1352,14 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       s[mt][0] += s2[mt][0]; s[mt][1] += s2[mt][1]; s[mt][2] += s2[mt][2]; s[mt][3] += s2[mt][3];
     }
     // s[mt] = { (key 16mt+g, q 2c), (key 16mt+g, q 2c+1), (key 16mt+g+8, q 2c), (key 16mt+g+8, q 2c+1) }
+
+    if constexpr (I8) {
+#pragma unroll
+      for (int mt = 0; mt < NMT; ++mt) {
+        const float ka = sc_cur.key(mt * 16, g8), kb = sc_cur.key(mt * 16 + 8, g8);
+        s[mt][0] *= ka; s[mt][1] *= ka; s[mt][2] *= kb; s[mt][3] *= kb;
+      }
+    }
 
     // ---- mask (only tiles that touch a boundary)
     const int key_last = key0 + TILE_N - 1;
@@ -1271,6 +1403,19 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       m0 = mn0;
       m1 = mn1;
     }
+    if constexpr (I8) {
+      const float vmax = sc_cur.max_val();
+      if (vmax > vref) {   // (warp-uniform) O is kept in units of the largest V scale
+        const float f = vref / vmax;
+#pragma unroll
+        for (int i = 0; i < NDT; ++i) {
+          o[i][0] *= f; o[i][1] *= f; o[i][2] *= f; o[i][3] *= f;
+        }
+        vref = vmax;
+        vinv = kVScaleUp / vmax;
+        vscale = vmax * (1.f / kVScaleUp);
+      }
+    }
     const float ms0 = (m0 == -INFINITY) ? 0.f : m0 * sl2;
     const float ms1 = (m1 == -INFINITY) ? 0.f : m1 * sl2;
     uint32_t pb[NMT][2];  // P^T B fragments per 16-key block
@@ -1282,8 +1427,10 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       const float p3 = ex2(fmaf(s[mt][3], sl2, -ms1));
       l0 += p0 + p2;
       l1 += p1 + p3;
-      pb[mt][0] = movmatrix_trans(pack2<BF16>(p0, p1));  // (keys 16mt+2c, +1 ; q g)
-      pb[mt][1] = movmatrix_trans(pack2<BF16>(p2, p3));  // (keys 16mt+8+2c, +1 ; q g)
+      float va = 1.f, vb = 1.f;
+      if constexpr (I8) { va = sc_cur.val(mt * 16, g8) * vinv; vb = sc_cur.val(mt * 16 + 8, g8) * vinv; }
+      pb[mt][0] = movmatrix_trans(I8 ? pack2<BF16>(p0 * va, p1 * va) : pack2<BF16>(p0, p1));  // (keys 16mt+2c, +1 ; q g)
+      pb[mt][1] = movmatrix_trans(I8 ? pack2<BF16>(p2 * vb, p3 * vb) : pack2<BF16>(p2, p3));  // (keys 16mt+8+2c, +1 ; q g)
     }
 
     // ---- O^T += V^T P^T.  Rows of V past the sequence end may hold anything (NaN bit
@@ -1319,28 +1466,33 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             ldsm_x4_t(x0, x1, x2, x3, addr);
             if constexpr (MASKED) { x0 &= mk_lo; x1 &= mk_hi; x2 &= mk_lo; x3 &= mk_hi; }
             // word = [key 2c: d, d+1 | key 2c+1: d, d+1]  ->  [d: key 2c, 2c+1 | d+1: key 2c, 2c+1]
-            x0 = __byte_perm(x0, 0, 0x3120);
-            x1 = __byte_perm(x1, 0, 0x3120);
-            x2 = __byte_perm(x2, 0, 0x3120);
-            x3 = __byte_perm(x3, 0, 0x3120);
+            if constexpr (!I8) {   // (the int8 conversion pairs bytes 0, 2 and 1, 3 as it is)
+              x0 = __byte_perm(x0, 0, 0x3120);
+              x1 = __byte_perm(x1, 0, 0x3120);
+              x2 = __byte_perm(x2, 0, 0x3120);
+              x3 = __byte_perm(x3, 0, 0x3120);
+            }
             uint32_t a0, a1, a2, a3;
-            e4m3x4_to_f16x4(x0, a0, a1);  // row g: d = 16ch + 2g ; row g+8: d = 16ch + 2g + 1 (keys lo)
-            e4m3x4_to_f16x4(x1, a2, a3);  // same rows, keys hi
+            widen(x0, a0, a1);  // row g: d = 16ch + 2g ; row g+8: d = 16ch + 2g + 1 (keys lo)
+            widen(x1, a2, a3);  // same rows, keys hi
             mma16816r<false>(o[2 * cp], a0, a1, a2, a3, pb[mt][0], pb[mt][1]);
-            e4m3x4_to_f16x4(x2, a0, a1);
-            e4m3x4_to_f16x4(x3, a2, a3);
+            widen(x2, a0, a1);
+            widen(x3, a2, a3);
             mma16816r<false>(o[2 * cp + 1], a0, a1, a2, a3, pb[mt][0], pb[mt][1]);
           }
         }
       }
     };
-    if (key0 + TILE_N > cc.L) pv(std::true_type{});
+    // (int8 codes are numbers whatever they are, and the weights of keys past the end are zero)
+    if (!I8 && key0 + TILE_N > cc.L) pv(std::true_type{});
     else pv(std::false_type{});
 
     // ---- this stage has been read: refill it with the tile NS ahead
     __syncwarp();
+    if constexpr (I8) sc_cur = sc_next;
     if (prod.more()) {
       fence_proxy_async();
+      if constexpr (I8) prod.fetch_scales(sc_next);
       prod.issue(stage);
     }
 
@@ -1405,6 +1557,12 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         const int64_t slot = (int64_t)(cc.segbase + cc.seg) + w;
         float* po = p.part_o + slot * (kRowsPerSeg * HD);
         float* pml = p.part_ml + slot * (kRowsPerSeg * 2);
+        if constexpr (I8) {   // (the merge multiplies by a scale that is 1 for such pools)
+#pragma unroll
+          for (int i = 0; i < NDT; ++i) {
+            o[i][0] *= vscale; o[i][1] *= vscale; o[i][2] *= vscale; o[i][3] *= vscale;
+          }
+        }
         const int rl0 = 2 * c4, rl1 = rl0 + 1;  // row inside the segment
         // (rows past the segment's end are neither written here nor read by the merge)
         const int nrows_seg = p.group * cc.sq - mb * kDecodeRows;
@@ -1643,7 +1801,7 @@ inline int get_pool_tmap(const TmapKey& key_in, int tile_n, bool merged, CUtenso
                            (cuuint64_t)(key.page_stride * es)};
   cuuint32_t box[4] = {(cuuint32_t)(rb / es), (cuuint32_t)box_rows, 1u, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-  CUtensorMapDataType dt = key.dtype == KB200_DTYPE_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+  CUtensorMapDataType dt = dtype_size(key.dtype) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                            : key.dtype == KB200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMapSwizzle sw = rb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
@@ -1732,11 +1890,11 @@ inline int device_sm_count(int dev, int* sms) {
   return KB200_OK;
 }
 
-template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER>
+template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER, bool I8 = false>
 inline int launch_attn_variant(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
                                int dev, cudaStream_t stream) {
   using T = AttnTile<KVB, HD, NW, NS>;
-  auto kern = paged_attn_kernel<KVB, HD, BF16, NW, NS, GATHER>;
+  auto kern = paged_attn_kernel<KVB, HD, BF16, NW, NS, GATHER, I8>;
   static SmemAttrOnce once;
   static_assert(T::SMEM_BYTES + plan_smem_bytes(kPlanSmemMaxBatch) <= 232448, "shared memory of the largest in-kernel plan");
   if (int rc = once.ensure(kern, T::SMEM_BYTES + plan_smem_bytes(kPlanSmemMaxBatch), dev)) return rc;
@@ -1745,11 +1903,11 @@ inline int launch_attn_variant(const CUtensorMap& tmK, const CUtensorMap& tmV, c
   return KB200_OK;
 }
 
-template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER>
+template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER, bool I8 = false>
 inline int launch_decode_variant(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
                                  int dev, cudaStream_t stream) {
   using T = AttnTile<KVB, HD, NW, NS>;
-  auto kern = paged_attn_decode_kernel<KVB, HD, BF16, NW, NS, GATHER>;
+  auto kern = paged_attn_decode_kernel<KVB, HD, BF16, NW, NS, GATHER, I8>;
   static SmemAttrOnce once;
   static_assert(T::SMEM_BYTES + plan_smem_bytes(kPlanSmemMaxBatch) <= 232448, "shared memory of the largest in-kernel plan");
   if (int rc = once.ensure(kern, T::SMEM_BYTES + plan_smem_bytes(kPlanSmemMaxBatch), dev)) return rc;
@@ -1758,11 +1916,11 @@ inline int launch_decode_variant(const CUtensorMap& tmK, const CUtensorMap& tmV,
   return KB200_OK;
 }
 
-template <int KVB, int HD, bool BF16, bool GATHER>
+template <int KVB, int HD, bool BF16, bool GATHER, bool I8 = false>
 inline int launch_rows32_variant(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
                                  int dev, cudaStream_t stream) {
   using L = Rows32Smem<KVB, HD, 2>;
-  auto kern = paged_attn_rows32_kernel<KVB, HD, BF16, 2, GATHER>;
+  auto kern = paged_attn_rows32_kernel<KVB, HD, BF16, 2, GATHER, I8>;
   static SmemAttrOnce once;
   static_assert(L::SMEM_BYTES + plan_smem_bytes(kPlanSmemMaxBatch) <= 232448, "shared memory of the largest in-kernel plan");
   if (int rc = once.ensure(kern, L::SMEM_BYTES + plan_smem_bytes(kPlanSmemMaxBatch), dev)) return rc;
@@ -1808,6 +1966,18 @@ inline int launch_attn_hd(int nw, const CUtensorMap& tmK, const CUtensorMap& tmV
   }
 }
 
+// int8 pools: the e4m3 geometry of each kernel
+template <int HD>
+inline int launch_i8_hd(bool decode8, bool rows32, const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
+                        int dev, cudaStream_t stream) {
+  if (rows32) return p.gather ? launch_rows32_variant<1, HD, false, true, true>(tmK, tmV, p, grid, dev, stream)
+                              : launch_rows32_variant<1, HD, false, false, true>(tmK, tmV, p, grid, dev, stream);
+  if (decode8) return p.gather ? launch_decode_variant<1, HD, false, 12, 2, true, true>(tmK, tmV, p, grid, dev, stream)
+                               : launch_decode_variant<1, HD, false, 12, 2, false, true>(tmK, tmV, p, grid, dev, stream);
+  return p.gather ? launch_attn_variant<1, HD, false, 12, 2, true, true>(tmK, tmV, p, grid, dev, stream)
+                  : launch_attn_variant<1, HD, false, 12, 2, false, true>(tmK, tmV, p, grid, dev, stream);
+}
+
 template <int KVB, bool BF16>
 inline int launch_attn_dispatch(bool d128, int nw, const CUtensorMap& tmK, const CUtensorMap& tmV,
                                 const AttnParams& p, int grid, int dev, cudaStream_t stream) {
@@ -1815,9 +1985,22 @@ inline int launch_attn_dispatch(bool d128, int nw, const CUtensorMap& tmK, const
               : launch_attn_hd<KVB, BF16, 64>(nw, tmK, tmV, p, grid, dev, stream);
 }
 
+inline bool kv_is_8bit(int dtype) { return dtype == KB200_DTYPE_E4M3 || dtype == KB200_DTYPE_I8; }
+
+// The call's arguments with every field this build has: a caller built before the int8 pools passes the smaller struct
+// (its last fields then are null).  False for any other size.
+inline bool attn_args_in_full(const kb200_attn_args* given, kb200_attn_args* out) {
+  constexpr uint32_t kBefore = (uint32_t)offsetof(kb200_attn_args, k_block_scale);
+  if (given->struct_bytes != sizeof(kb200_attn_args) && given->struct_bytes != kBefore) return false;
+  memset(out, 0, sizeof(*out));
+  memcpy(out, given, given->struct_bytes);
+  out->struct_bytes = sizeof(kb200_attn_args);
+  return true;
+}
+
 // paged_prefill.cuh
 bool prefill_enabled();
-template <int HD, bool BF16, bool KV8>
+template <int HD, bool BF16, bool KV8, bool I8 = false>
 int launch_prefill_variant(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid, int dev,
                            cudaStream_t stream);
 constexpr int kPrefillRowsPerSeg = 256, kPrefillTileKeys = 128, kPrefillMinPackedRows = 64;
@@ -1840,6 +2023,7 @@ constexpr int kPrefillRowsPerSeg = 256, kPrefillTileKeys = 128, kPrefillMinPacke
 //     with it: 40 rows: 256 x U[2k,16k] 1.77 | 2.39, 16 x: 0.206 | 0.171; 64 rows: 1.78 | 2.44, 0.204 | 0.179;
 //       128 rows: 256 x 1.83, 16 x 0.210                            -> 33 once there is a CTA per SM (32 rows and
 //       fewer stay with the 32-row kernel, which reads the keys once as well and spreads them over all SMs)
+// (int8 pools: the e4m3 rules)
 inline int prefill_min_rows(bool kv8) { return kv8 ? 65 : 33; }
 
 // A TMA box must fill a multiple of 128 bytes of shared memory: page_size x min(row bytes, 128).  Pools
@@ -1864,7 +2048,7 @@ inline bool use_prefill_kernel(const kb200_attn_args* a) {
   int64_t rows = a->seqlen_q;
   if (a->cu_seqlens_q && a->batch > 0) rows = std::min<int64_t>(rows, (a->total_q + a->batch - 1) / a->batch);
   const int64_t packed_rows = (int64_t)(a->n_q_heads / a->n_kv_heads) * rows;
-  const bool kv8 = a->kv_dtype == KB200_DTYPE_E4M3;
+  const bool kv8 = kv_is_8bit(a->kv_dtype);
   if (packed_rows >= prefill_min_rows(kv8)) return true;
   // 17 .. 32 rows (33 .. 64 on e4m3 pools): with a CTA per SM at least, and only when the launch will get the
   // key-split variant (seqlen_q bounds every sequence's rows; a packed call without a bound keeps the 32-row kernel)
@@ -1886,6 +2070,7 @@ inline bool use_prefill_kernel(const kb200_attn_args* a) {
 // at most 8 packed rows for the wide head.  Returns the number of heads per pack (1: none).
 inline int attn_head_pack(const kb200_attn_args* a) {
   const bool kv8 = a->kv_dtype == KB200_DTYPE_E4M3;
+  if (a->kv_dtype == KB200_DTYPE_I8) return 1;   // (a scale per head: the heads of a pack would need one each per column)
   if (a->page_size > 2 || (kv8 && (a->k_scale_per_head || a->v_scale_per_head))) return 1;
   if (a->q_visible_until != nullptr || a->n_kv_heads <= 0) return 1;
   // wide rows of 256 bytes: four e4m3 heads of 64, two of 128, or two 16-bit heads of 64 (the reference's default
@@ -2125,8 +2310,10 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
   KB200_REQUIRE(a->q && a->out && a->k_cache && a->v_cache && a->page_table && (a->seqused_k || fixed_klen >= 0),
                 "null pointer argument");
   KB200_REQUIRE(a->q_dtype == KB200_DTYPE_F16 || a->q_dtype == KB200_DTYPE_BF16, "q must be F16 or BF16");
-  KB200_REQUIRE(a->kv_dtype == KB200_DTYPE_E4M3 || a->kv_dtype == a->q_dtype,
-                "K/V dtype must equal q dtype or be E4M3");
+  KB200_REQUIRE(kv_is_8bit(a->kv_dtype) || a->kv_dtype == a->q_dtype, "K/V dtype must equal q dtype or be E4M3 or I8");
+  const bool i8 = a->kv_dtype == KB200_DTYPE_I8;
+  KB200_REQUIRE(!i8 || (a->k_block_scale && a->v_block_scale), "int8 pools need k_block_scale and v_block_scale");
+  KB200_REQUIRE(!i8 || a->block_scale_page_stride >= a->n_kv_heads, "block_scale_page_stride is smaller than n_kv_heads");
   if (a->head_dim != 64 && a->head_dim != 128)
     return fail(KB200_ERR_UNSUPPORTED, "head_dim %d is not supported (64 or 128)", a->head_dim);
   KB200_REQUIRE(a->n_kv_heads > 0 && a->n_q_heads > 0 && a->n_q_heads % a->n_kv_heads == 0,
@@ -2165,11 +2352,11 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
   // on its own dependent MMA / ALU chains there, 45 % of the DRAM rate on short contexts).  16-bit K/V with
   // head_dim 128 is within a few percent of the HBM roofline with the 16-row kernel already.
   const bool decode8 = !prefill && (int64_t)group * a->seqlen_q <= kDecodeRows &&
-                       (a->kv_dtype == KB200_DTYPE_E4M3 || hd == 64 || pack > 1);
+                       (kv_is_8bit(a->kv_dtype) || hd == 64 || pack > 1);
   // (12 warps x 2 stages; 8 x 3 and 6 x 4 -- more tiles in flight per warp, fewer warps -- measured 2 % and
   // 13 % slower on the short contexts of a shared-prefix batch)
   const bool rows32 = use_rows32_kernel(a);   // (8 warps: two output accumulators per thread need the registers)
-  const int nw = rows32 ? 8 : (a->kv_dtype == KB200_DTYPE_E4M3 || decode8) ? 12 : 8;
+  const int nw = rows32 ? 8 : (kv_is_8bit(a->kv_dtype) || decode8) ? 12 : 8;
   const int n_workers = grid * nw;
   const AttnWorkspace wl = attn_workspace_layout(a->batch, a->total_q, a->n_q_heads, hkv, hd, grid * kAttnMaxWarps, rows32);
   const uint64_t ws_need = attn_pass_workspace_need(a, sms);
@@ -2274,6 +2461,9 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
   p.kv_ps_b = a->kv_page_stride * es;
   p.kv_ts_b = a->kv_token_stride * es;
   p.kv_hs_b = a->kv_head_stride * es * pack;
+  p.kbs = i8 ? a->k_block_scale : nullptr;
+  p.vbs = i8 ? a->v_block_scale : nullptr;
+  p.bs_ps = i8 ? a->block_scale_page_stride : 0;
   // the split-KV kernels build the plan themselves (every CTA, into shared memory) unless the batch is too large
   p.plan_in_kernel = (!prefill && a->batch <= kPlanSmemMaxBatch) ? 1 : 0;
 
@@ -2291,7 +2481,12 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
                                 : a->batch * (int64_t)a->n_kv_heads * ((group * (int64_t)a->seqlen_q + kPrefillRowsPerSeg - 1) / kPrefillRowsPerSeg);
     KB200_REQUIRE(nseg <= 0x7fffffff, "too many segments");
     const bool bf = a->q_dtype == KB200_DTYPE_BF16;
-    if (a->kv_dtype == KB200_DTYPE_E4M3) {
+    if (i8) {
+      if (d128) rc = bf ? launch_prefill_variant<128, true, true, true>(tmK, tmV, p, (int)nseg, a->device, stream)
+                        : launch_prefill_variant<128, false, true, true>(tmK, tmV, p, (int)nseg, a->device, stream);
+      else rc = bf ? launch_prefill_variant<64, true, true, true>(tmK, tmV, p, (int)nseg, a->device, stream)
+                   : launch_prefill_variant<64, false, true, true>(tmK, tmV, p, (int)nseg, a->device, stream);
+    } else if (a->kv_dtype == KB200_DTYPE_E4M3) {
       if (d128) rc = bf ? launch_prefill_variant<128, true, true>(tmK, tmV, p, (int)nseg, a->device, stream)
                         : launch_prefill_variant<128, false, true>(tmK, tmV, p, (int)nseg, a->device, stream);
       else rc = bf ? launch_prefill_variant<64, true, true>(tmK, tmV, p, (int)nseg, a->device, stream)
@@ -2304,7 +2499,10 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
     }
     return rc;   // every segment is written by its own CTA: nothing to merge
   }
-  if (pack > 1 && a->kv_dtype == KB200_DTYPE_E4M3)   // (gather, at most 8 rows: the transposed kernel on the wide head)
+  if (i8)
+    rc = d128 ? launch_i8_hd<128>(decode8, rows32, tmK, tmV, p, grid, a->device, stream)
+              : launch_i8_hd<64>(decode8, rows32, tmK, tmV, p, grid, a->device, stream);
+  else if (pack > 1 && a->kv_dtype == KB200_DTYPE_E4M3)   // (gather, at most 8 rows: the transposed kernel on the wide head)
     rc = launch_decode_variant<1, 256, false, 12, 2, true>(tmK, tmV, p, grid, a->device, stream);
   else if (pack > 1)
     rc = a->kv_dtype == KB200_DTYPE_BF16 ? launch_decode_variant<2, 128, true, 12, 2, true>(tmK, tmV, p, grid, a->device, stream)

@@ -24,7 +24,7 @@ struct Rows32Smem {
   static constexpr int SMEM_BYTES = PLAN_OFF + 1024;   // + plan_smem_bytes(batch) at launch
 };
 
-template <int KVB, int HD, bool BF16, int NS, bool GATHER>
+template <int KVB, int HD, bool BF16, int NS, bool GATHER, bool I8 = false>
 __global__ void __launch_bounds__(256, 1)
 paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                          const __grid_constant__ AttnParams p) {
@@ -77,7 +77,15 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   TileProducer<T, KVB, GATHER> prod(p, plan, &tmK, &tmV, my_stage0, bar0, lane, r0, my_tiles);
   Cursor cc = prod.pc;   // consumer side: starts where the producer starts
   if (lane == 0 && w > 0) write_boundary_record(p, w, cc);
-  for (int s = 0; s < NS && prod.more(); ++s) prod.issue(s);
+  [[maybe_unused]] TileScales<(TILE_N + 31) / 32> sc_cur, sc_next;   // (I8) scales of the tile being read and of the next one
+  if constexpr (I8) {
+    static_assert(KVB == 1 && NS == 2, "two tiles' scales are kept");
+    prod.fetch_scales(sc_cur);
+    prod.issue(0);
+    if (prod.more()) { prod.fetch_scales(sc_next); prod.issue(1); }
+  } else {
+    for (int s = 0; s < NS && prod.more(); ++s) prod.issue(s);
+  }
 
   // Lane-dependent parts of the ldmatrix addresses.  A 16-byte chunk c of row r sits at chunk (c & 8) |
   // ((c & 7) ^ (r & 7)); c = (even constant of the unrolled loop) + (a lane bit), r & 7 = lane & 7 everywhere, so
@@ -98,6 +106,7 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   int lim[2][2], rowi[2][2];
   bool valid[2][2];
   float sl2 = 0.f, lazy = 0.f, vscale = 1.f;
+  [[maybe_unused]] float vref = 0.f, vinv = 0.f;   // (I8) largest V scale seen, and what a V scale is multiplied by
   int h = 0;
   bool two = false;            // the second block has rows at all (warp-uniform)
   bool fresh = true;
@@ -129,6 +138,7 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       }
       const float ksc = p.ks_vec ? p.ks_vec[h] : p.ks;
       vscale = p.vs_vec ? p.vs_vec[h] : p.vs;
+      if constexpr (I8) { vref = vinv = 0.f; }
       sl2 = p.softmax_scale * ksc * kLog2e;
       lazy = 8.f / sl2;
 
@@ -161,6 +171,7 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             v.z = pack2<false>(bf16_bits_to_float(v.z & 0xffffu), bf16_bits_to_float(v.z >> 16));
             v.w = pack2<false>(bf16_bits_to_float(v.w & 0xffffu), bf16_bits_to_float(v.w >> 16));
           }
+          if constexpr (I8) { pair_02_13(v.x, v.y); pair_02_13(v.z, v.w); }   // (4c + {0, 2} and 4c + {1, 3} there)
           const int grp = gc >> 1, byte = 8 * (gc & 1);
           const int ca = 2 * grp, cb = 2 * grp + 1;
           *reinterpret_cast<uint2*>(row + (((ca & ~7) | ((ca & 7) ^ (r & 7))) << 4) + byte) = make_uint2(v.x, v.z);
@@ -185,6 +196,10 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       return q_lane + q_x[ks & 3] + (uint32_t)(blk * 16 * L::Q_ROW_BYTES + ((2 * ks) & 8) * 16);
     };
 
+    auto widen = [](uint32_t x, uint32_t& e, uint32_t& o_) {
+      if constexpr (I8) i8x4_to_f16x4(x, e, o_);
+      else e4m3x4_to_f16x4(x, e, o_);
+    };
     // ---- S = Q K^T for both blocks; every K fragment is loaded (and widened) once
     float s[2][NT8][4];
 #pragma unroll
@@ -232,12 +247,12 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             uint32_t x0, x1;
             ldsm_x2(x0, x1, addr);
             uint32_t b0, b1;
-            e4m3x4_to_f16x4(x0, b0, b1);
+            widen(x0, b0, b1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(s[blk][n], qa[blk][0], b0, b1);
             }
-            e4m3x4_to_f16x4(x1, b0, b1);
+            widen(x1, b0, b1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(s[blk][n], qa[blk][1], b0, b1);
@@ -252,6 +267,29 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     const int min_lim = (p.causal || p.window_left >= 0) ? cc.L - cc.sq : cc.L - 1;
     const bool need_mask = key_last > min_lim || (p.window_left >= 0 && key0 < cc.L - 1 - p.window_left);
     uint32_t pf[2][NKS][4];
+    if constexpr (I8) {
+#pragma unroll
+      for (int n = 0; n < NT8; ++n) {
+        const float ka = sc_cur.key(n * 8, 2 * c4), kb = sc_cur.key(n * 8, 2 * c4 + 1);
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+          s[blk][n][0] *= ka; s[blk][n][1] *= kb; s[blk][n][2] *= ka; s[blk][n][3] *= kb;
+        }
+      }
+      const float vmax = sc_cur.max_val();
+      if (vmax > vref) {   // (warp-uniform) O is kept in units of the largest V scale
+        const float f = vref / vmax;
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+          for (int i = 0; i < NOT; ++i) {
+            o[blk][i][0] *= f; o[blk][i][1] *= f; o[blk][i][2] *= f; o[blk][i][3] *= f;
+          }
+        vref = vmax;
+        vinv = kVScaleUpLazy / vmax;
+        vscale = vmax * (1.f / kVScaleUpLazy);
+      }
+    }
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
       if (need_mask) {
@@ -303,8 +341,14 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         const float p3 = ex2(fmaf(s[blk][n][3], sl2, -ms1));
         ls[blk][0] += p0 + p1;
         ls[blk][1] += p2 + p3;
-        pf[blk][n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0, p1);
-        pf[blk][n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2, p3);
+        if constexpr (I8) {
+          const float va = sc_cur.val(n * 8, 2 * c4) * vinv, vb = sc_cur.val(n * 8, 2 * c4 + 1) * vinv;
+          pf[blk][n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0 * va, p1 * vb);
+          pf[blk][n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2 * va, p3 * vb);
+        } else {
+          pf[blk][n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0, p1);
+          pf[blk][n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2, p3);
+        }
       }
     }
 
@@ -343,20 +387,22 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             ldsm_x4_t(x0, x1, x2, x3, addr);
             if constexpr (MASKED) { x0 &= mk_lo; x1 &= mk_hi; x2 &= mk_lo; x3 &= mk_hi; }
             // word = [key 2c: d, d+1 | key 2c+1: d, d+1]  ->  [d: key 2c, 2c+1 | d+1: key 2c, 2c+1]
-            x0 = __byte_perm(x0, 0, 0x3120);
-            x1 = __byte_perm(x1, 0, 0x3120);
-            x2 = __byte_perm(x2, 0, 0x3120);
-            x3 = __byte_perm(x3, 0, 0x3120);
+            if constexpr (!I8) {   // (the int8 conversion pairs bytes 0, 2 and 1, 3 as it is)
+              x0 = __byte_perm(x0, 0, 0x3120);
+              x1 = __byte_perm(x1, 0, 0x3120);
+              x2 = __byte_perm(x2, 0, 0x3120);
+              x3 = __byte_perm(x3, 0, 0x3120);
+            }
             uint32_t e0, o0, e1, o1;
-            e4m3x4_to_f16x4(x0, e0, o0);
-            e4m3x4_to_f16x4(x1, e1, o1);
+            widen(x0, e0, o0);
+            widen(x1, e1, o1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(o[blk][4 * q2 + 0], pf[blk][ks], e0, e1);  // d = 16*(2*q2)   + 2g
               mma16816<false>(o[blk][4 * q2 + 1], pf[blk][ks], o0, o1);  // d = 16*(2*q2)   + 2g + 1
             }
-            e4m3x4_to_f16x4(x2, e0, o0);
-            e4m3x4_to_f16x4(x3, e1, o1);
+            widen(x2, e0, o0);
+            widen(x3, e1, o1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(o[blk][4 * q2 + 2], pf[blk][ks], e0, e1);  // d = 16*(2*q2+1) + 2g
@@ -366,13 +412,16 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         }
       }
     };
-    if (key0 + TILE_N > cc.L) pv(std::true_type{});
+    // (int8 codes are numbers whatever they are, and the weights of keys past the end are zero)
+    if (!I8 && key0 + TILE_N > cc.L) pv(std::true_type{});
     else pv(std::false_type{});
 
     // ---- this stage has been read: refill it with the tile NS ahead
     __syncwarp();
+    if constexpr (I8) sc_cur = sc_next;
     if (prod.more()) {
       fence_proxy_async();
+      if constexpr (I8) prod.fetch_scales(sc_next);
       prod.issue(stage);
     }
 
@@ -436,6 +485,12 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           const int64_t slot = ((int64_t)seg_id + w) * 2 + blk;
           float* po = p.part_o + slot * (kRowsPerSeg * HD);
           float* pml = p.part_ml + slot * (kRowsPerSeg * 2);
+          if constexpr (I8) {   // (the merge multiplies by a scale that is 1 for such pools)
+#pragma unroll
+            for (int i = 0; i < NOT; ++i) {
+              o[blk][i][0] *= vscale; o[blk][i][1] *= vscale; o[blk][i][2] *= vscale; o[blk][i][3] *= vscale;
+            }
+          }
           const bool wv0 = valid[blk][0], wv1 = valid[blk][1];   // rows past the end: not written, not read by the merge
           if (c4 == 0) {
             if (wv0) *reinterpret_cast<float2*>(pml + g8 * 2) = make_float2((m0 == -INFINITY) ? -INFINITY : m0 * sl2, l0);

@@ -216,17 +216,34 @@ __host__ __device__ constexpr uint32_t umma_idesc(bool bf16, bool b_mn_major, in
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPfTileRows >> 4) << 24);
 }
 
+// Four int8 codes -> (code + 1/2) * s in the operand type.  A byte, its sign flipped, dropped into bits 8-15 of 2^15 is
+// 2^15 + 128 + code in fp32; one fma by s and off = -(2^15 + 127.5) s does the rest exactly (s a power of two).
+template <bool BF16>
+__device__ __forceinline__ void i8x4_scaled(uint32_t x, float s, float off, uint32_t& lo, uint32_t& hi) {
+  x ^= 0x80808080u;
+  const float a = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7604)), s, off);
+  const float b = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7614)), s, off);
+  const float c = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7624)), s, off);
+  const float d = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7634)), s, off);
+  lo = pack2<BF16>(a, b);
+  hi = pack2<BF16>(c, d);
+}
+
 // BF16: dtype of q and out.  KV8: K/V pools hold e4m3 codes; the tiles are widened to f16 in shared memory
 // (exact), the tensor core then runs on f16 operands (q is converted once, as in the decode kernels)
 // and the dequantisation scales are folded into the softmax scale (K) and the final normalisation (V).
 // SPLIT: no sequence of the launch brings more than 128 packed rows per KV head, so no CTA has rows in its
 // second Q tile and the key split (below) is open to every CTA; the ring then has one slot more.
-template <int HD, bool BF16, bool KV8, bool SPLIT>
+// I8: the pools hold int8 codes with a scale per (page, head) instead.  (code + 1/2) * scale has eight significant bits and,
+// with the scales the append makes, is exact in bf16 over all of its range (in f16 down to its last place, 2^-24): the
+// widening warps write finished values in q's own type and nothing of the scales is left for the softmax.
+template <int HD, bool BF16, bool KV8, bool SPLIT, bool I8 = false>
 __global__ void __launch_bounds__(pf_threads(KV8), 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ AttnParams p) {
   using SM = PrefillSmem<HD, KV8>;
-  constexpr bool MMA_BF16 = BF16 && !KV8;   // operand type of both products
+  static_assert(!I8 || KV8, "int8 tiles are widened like e4m3 tiles");
+  constexpr bool MMA_BF16 = BF16 && (!KV8 || I8);   // operand type of both products
   constexpr int NH = SM::NH;
   constexpr int RING = SM::RING;
   // Under the key split Q tile B is unused and lies directly below the K/V ring: it becomes one more ring slot
@@ -404,7 +421,32 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     constexpr int RB8 = SM::RB8;
     constexpr int NSTG = SM::NSTG > 0 ? SM::NSTG : 1;   // (this branch is only taken with a staging ring)
     const int r = (warp - 10) * 32 + lane;
+    // (I8) scales of this row's key, fetched a tile ahead: table entry, then scales, are dependent loads
+    [[maybe_unused]] float sk = 0.f, sv = 0.f, sk_next = 0.f, sv_next = 0.f;
+    [[maybe_unused]] int page_next = -1;
+    [[maybe_unused]] auto page_of = [&](int tile) -> int {
+      const int key = (tile_begin + tile) * BN + r;
+      return tile < n_tiles && key < L ? p.page_table[pt_row + (key >> p_shift)] : -1;
+    };
+    [[maybe_unused]] auto scale_at = [&](const float* scales, int page) -> float {
+      return (unsigned)page < (unsigned long long)p.n_pages ? scales[page * p.bs_ps + h] : 0.f;   // (-1: past the end)
+    };
+    if constexpr (I8) {
+      const int pg0 = page_of(0);
+      page_next = page_of(1);
+      sk_next = scale_at(p.kbs, pg0);
+      sv_next = scale_at(p.vbs, pg0);
+    }
     for (int idx = 0; idx < 2 * n_tiles; ++idx) {
+      if constexpr (I8) {
+        if ((idx & 1) == 0) {   // a new tile: its scales have arrived, the next tile's are asked for
+          sk = sk_next;
+          sv = sv_next;
+          sk_next = scale_at(p.kbs, page_next);
+          sv_next = scale_at(p.vbs, page_next);
+          page_next = page_of((idx >> 1) + 2);
+        }
+      }
       const int s8 = idx % NSTG, c = idx % RINGN;
       bool got = mbar_wait_bounded(B_SFULL(s8), (uint32_t)(idx / NSTG) & 1u);
       if (got && idx >= RINGN) got = mbar_wait_bounded(B_EMPTY(c), (uint32_t)((idx / RINGN) - 1) & 1u);
@@ -417,11 +459,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 #pragma unroll
       for (int ch = 0; ch < RB8 / 16; ++ch) {
         const uint4 x = *reinterpret_cast<const uint4*>(src + ((ch ^ (int)swz<RB8>(r)) << 4));
-        uint4 lo4, hi4;   // elements 16ch .. 16ch+7 and 16ch+8 .. 16ch+15 as f16
-        e4m3x4_to_f16x4(x.x, lo4.x, lo4.y);
-        e4m3x4_to_f16x4(x.y, lo4.z, lo4.w);
-        e4m3x4_to_f16x4(x.z, hi4.x, hi4.y);
-        e4m3x4_to_f16x4(x.w, hi4.z, hi4.w);
+        uint4 lo4, hi4;   // elements 16ch .. 16ch+7 and 16ch+8 .. 16ch+15 as f16 (I8: in q's type)
+        if constexpr (I8) {
+          const float s = (idx & 1) ? sv : sk, off = -32895.5f * s;
+          i8x4_scaled<MMA_BF16>(x.x, s, off, lo4.x, lo4.y);
+          i8x4_scaled<MMA_BF16>(x.y, s, off, lo4.z, lo4.w);
+          i8x4_scaled<MMA_BF16>(x.z, s, off, hi4.x, hi4.y);
+          i8x4_scaled<MMA_BF16>(x.w, s, off, hi4.z, hi4.w);
+        } else {
+          e4m3x4_to_f16x4(x.x, lo4.x, lo4.y);
+          e4m3x4_to_f16x4(x.y, lo4.z, lo4.w);
+          e4m3x4_to_f16x4(x.z, hi4.x, hi4.y);
+          e4m3x4_to_f16x4(x.w, hi4.z, hi4.w);
+        }
         const int d0 = 2 * ch, d1 = 2 * ch + 1;   // 16-byte chunks of the f16 row
         *reinterpret_cast<uint4*>(dst + (d0 >> 3) * (BN * 128) + (((d0 & 7) ^ (r & 7)) << 4)) = lo4;
         *reinterpret_cast<uint4*>(dst + (d1 >> 3) * (BN * 128) + (((d1 & 7) ^ (r & 7)) << 4)) = hi4;
@@ -455,7 +505,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const char* src = p.q + 2 * ((int64_t)b * p.q_bs + (int64_t)(qrow0 + j) * p.q_rs +
                                      (int64_t)(h * p.group + g) * p.q_hs) + 16 * c;
         val[u] = *reinterpret_cast<const uint4*>(src);
-        if constexpr (KV8 && BF16) {   // bf16 -> f16 (exact unless |q| > 65504 or below the f16 subnormals)
+        if constexpr (KV8 && BF16 && !I8) {   // bf16 -> f16 (exact unless |q| > 65504 or below the f16 subnormals)
           uint32_t* w32 = reinterpret_cast<uint32_t*>(&val[u]);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -941,25 +991,25 @@ inline bool prefill_enabled() {
   return on;
 }
 
-template <int HD, bool BF16, bool KV8, bool SPLIT>
+template <int HD, bool BF16, bool KV8, bool SPLIT, bool I8>
 inline int launch_prefill_split(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
                                 int dev, cudaStream_t stream) {
   using SM = PrefillSmem<HD, KV8>;
-  auto kern = paged_prefill_kernel<HD, BF16, KV8, SPLIT>;
+  auto kern = paged_prefill_kernel<HD, BF16, KV8, SPLIT, I8>;
   static SmemAttrOnce once;
   if (int rc = once.ensure(kern, SM::BYTES, dev)) return rc;
   KB200_CUDA_OK(launch_kernel(kern, dim3(grid), dim3(pf_threads(KV8)), SM::BYTES, stream, tmK, tmV, p));
   return KB200_OK;
 }
 
-template <int HD, bool BF16, bool KV8>
+template <int HD, bool BF16, bool KV8, bool I8>
 inline int launch_prefill_variant(const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
                                   int dev, cudaStream_t stream) {
   // seqlen_q bounds the rows of every sequence (padded and packed layouts alike): at most 128 packed rows per
   // KV head means no CTA of the launch uses its second Q tile, and the key-split variant serves it
   if ((long long)p.group * p.seqlen_q <= kPfTileRows)
-    return launch_prefill_split<HD, BF16, KV8, true>(tmK, tmV, p, grid, dev, stream);
-  return launch_prefill_split<HD, BF16, KV8, false>(tmK, tmV, p, grid, dev, stream);
+    return launch_prefill_split<HD, BF16, KV8, true, I8>(tmK, tmV, p, grid, dev, stream);
+  return launch_prefill_split<HD, BF16, KV8, false, I8>(tmK, tmV, p, grid, dev, stream);
 }
 
 }  // namespace kb200

@@ -20,7 +20,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import sys
-from typing import Any, Optional, Sequence
+from typing import Any, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -33,6 +33,9 @@ _TORCH_TO_DTYPE = {
     torch.float8_e4m3fn: _native.DTYPE_E4M3,
     torch.uint8: _native.DTYPE_E4M3,  # the reference passes FP8 pools viewed as uint8
 }
+
+
+_ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _require_cuda(name: str, t: torch.Tensor) -> int:
@@ -126,6 +129,163 @@ def reshape_and_cache_flash(key: torch.Tensor, value: torch.Tensor, key_cache: t
         key_cache.data_ptr(), value_cache.data_ptr(), ps, ts, hs,
         slot_mapping.data_ptr(), T, n_pages, P, H, D, in_dt, cache_dt,
         ks_ptr, vs_ptr, n_scales, dev, _stream(dev)))
+
+
+def reshape_and_cache_block_int8(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                                 value_cache: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+                                 slot_mapping: torch.Tensor) -> None:
+    """Append token rows to int8 pools with one scale per block, a block being one page of one KV head.
+
+    ``key, value [T, H_kv, D]`` fp32 / fp16 / bf16 (token stride free, heads and D compact, D a multiple of 16);
+    ``key_cache, value_cache`` the int8 ``[n_pages, P, H_kv, D]`` views; ``key_scales, value_scales`` fp32
+    ``[n_pages, H_kv]``, written together with the codes; ``slot_mapping int64 [T]``, negative slots skipped.
+
+    An element is ``(code + 1/2) * scale``; the scale is the power of two ``s`` with ``64 s <= max |x| < 128 s`` over the
+    block's rows, the code ``floor(x / s)``, so that an element is off by at most ``s / 2``.  A block whose first
+    token is written starts anew; a later, larger row raises the scale and shifts the codes already there.  The bytes do not
+    depend on how a block's tokens are split over calls.  The tokens of one block have to be neighbours in
+    ``slot_mapping``; of equal neighbouring slots the last one counts.  A NaN is stored as code 0, an infinity saturates
+    (``STATUS_NOT_FINITE``).
+    """
+    dev = _require_cuda("key", key)
+    for nm, t in (("value", value), ("key_cache", key_cache), ("value_cache", value_cache), ("key_scales", key_scales),
+                  ("value_scales", value_scales), ("slot_mapping", slot_mapping)):
+        if _require_cuda(nm, t) != dev:
+            raise ValueError(f"{nm} lives on a different device than key")
+    if key.ndim != 3 or value.ndim != 3 or key.shape != value.shape:
+        raise ValueError("key and value must both have shape [num_tokens, n_kv_heads, head_dim]")
+    T, H, D = key.shape
+    for nm, t in (("key", key), ("value", value)):
+        if t.stride(2) != 1 or t.stride(1) != D:
+            raise ValueError(f"{nm} must be compact across heads/head_dim; got stride={t.stride()}")
+    geometry = n_pages, P, Hc, Dc, ps, ts, hs = _cache_view_geometry("key_cache", key_cache)
+    if _cache_view_geometry("value_cache", value_cache) != geometry:
+        raise ValueError("key_cache and value_cache must have the same shape and strides")
+    if (Hc, Dc) != (H, D):
+        raise ValueError(f"cache heads/head_dim {(Hc, Dc)} do not match the rows {(H, D)}")
+    if key_cache.dtype != torch.int8 or value_cache.dtype != torch.int8:
+        raise ValueError(f"block-scaled caches must be int8, got {key_cache.dtype}/{value_cache.dtype}")
+    _check_block_scales(key_scales, value_scales, n_pages, H)
+    if key.dtype not in _ROW_DTYPES or value.dtype != key.dtype:
+        raise ValueError(f"unsupported row dtype {key.dtype}/{value.dtype}")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.ndim != 1 or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous 1-D int64 tensor")
+    if slot_mapping.numel() != T:
+        raise RuntimeError("slot_mapping size does not match the number of token rows")
+    if T == 0:
+        return
+    _native.check(_native.load().kb200_append_block_int8(
+        key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), key_cache.data_ptr(), value_cache.data_ptr(),
+        ps, ts, hs, key_scales.data_ptr(), value_scales.data_ptr(), key_scales.stride(0), slot_mapping.data_ptr(), T,
+        n_pages, P, H, D, _TORCH_TO_DTYPE[key.dtype], dev, _stream(dev)))
+
+
+def _check_block_scales(k: torch.Tensor, v: torch.Tensor, n_pages: int, n_heads: int) -> None:
+    for t in (k, v):
+        if t.dtype != torch.float32 or t.shape != (n_pages, n_heads) or t.stride(1) != 1:
+            raise ValueError(f"block scales must be fp32 [n_pages, n_kv_heads] = {(n_pages, n_heads)}, contiguous in the heads; "
+                             f"got {t.dtype} {tuple(t.shape)}")
+    if k.stride(0) != v.stride(0):
+        raise ValueError("the K and V block scales must have the same strides")
+    if n_pages > 1 and k.stride(0) < n_heads:
+        raise ValueError("block scales of different pages must not share memory")
+
+
+class RaggedStep(NamedTuple):
+    """What :func:`build_ragged_step` returns; all on the GPU."""
+
+    page_table: torch.Tensor      # int32 [B, >= pages]: the entries' rows, compact
+    seqused_k: torch.Tensor       # int32 [B]
+    cu_seqlens_q: torch.Tensor    # int32 [B + 1]
+    slot_mapping: torch.Tensor    # int64 [n_tokens], -1 behind the last token
+    positions: torch.Tensor       # int64 [n_tokens], 0 behind the last token
+    free_count: torch.Tensor      # int32 [1]
+    pages_taken: torch.Tensor     # int32 [1], -1: the step did not fit and took nothing
+
+
+def build_ragged_step(page_table: torch.Tensor, batch_idx: torch.Tensor, lengths: torch.Tensor, new_tokens: torch.Tensor,
+                      free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int, *, n_pages: int, n_tokens: int,
+                      out_page_table: torch.Tensor, out_seqused_k: Optional[torch.Tensor] = None,
+                      out_cu_seqlens_q: Optional[torch.Tensor] = None, out_slot_mapping: Optional[torch.Tensor] = None,
+                      out_positions: Optional[torch.Tensor] = None, out_free_count: Optional[torch.Tensor] = None,
+                      out_pages_taken: Optional[torch.Tensor] = None) -> RaggedStep:
+    """The tables of one ragged step from request lengths, in one launch and without the host: entry ``i`` (row
+    ``batch_idx[i]`` of ``page_table``) holds ``lengths[i]`` tokens and appends ``new_tokens[i]``.
+
+    Takes the pages the step needs from the end of ``free_pages[:free_count]`` (int32; the order of
+    ``PageTable.reserve`` called entry after entry), writes them into ``page_table`` (int32 ``[rows, cols]``), and returns the
+    compact block table (``out_page_table [B, cols]``, entries behind a row's last page untouched), ``seqused_k``,
+    packed row offsets, and for each of up to ``n_tokens`` packed tokens its slot and position.  Row 0 is the padding
+    row: it is never given pages.  ``batch_idx`` int32 / int64, distinct but for row 0; the other inputs int32.
+
+    ``out_seqused_k`` may be ``lengths`` and ``out_free_count`` may be ``free_count``: a captured step then advances its own
+    state.  All or nothing: a step that needs more pages than are free or more than ``n_tokens`` tokens takes nothing,
+    returns ``pages_taken = -1`` and no tokens (``STATUS_NO_PAGES``).  An entry whose row or counts are out of range
+    gets no tokens and ``seqused_k = 0`` (``STATUS_BAD_ROW``).
+    """
+    dev = _require_cuda("page_table", page_table)
+    B, n_tokens = batch_idx.shape[0], int(n_tokens)
+    for nm, t, n in (("lengths", lengths, B), ("new_tokens", new_tokens, B), ("free_pages", free_pages, 0),
+                     ("free_count", free_count, 1)):
+        if _require_cuda(nm, t) != dev or t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous():
+            raise ValueError(f"{nm} must be a contiguous int32 tensor of at least {n} elements on the page table's device")
+    if _require_cuda("batch_idx", batch_idx) != dev or batch_idx.ndim != 1 or not batch_idx.is_contiguous() \
+            or batch_idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError("batch_idx must be a contiguous 1-D int32/int64 tensor on the page table's device")
+    for nm, t in (("page_table", page_table), ("out_page_table", out_page_table)):
+        if _require_cuda(nm, t) != dev or t.dtype != torch.int32 or t.ndim != 2 or t.stride(1) != 1:
+            raise ValueError(f"{nm} must be int32 [rows, pages], contiguous in the last dimension, on one device")
+    if out_page_table.shape[0] < B:
+        raise ValueError("out_page_table has fewer rows than the batch")
+    if n_tokens < 0:
+        raise ValueError("n_tokens must not be negative")
+    ints = [out_seqused_k, out_cu_seqlens_q, out_free_count, out_pages_taken]
+    sizes = (B, B + 1, 1, 1)
+    if not any(t is not None for t in ints):   # (one buffer: a step of a few requests is bound by its host side)
+        ints = list(torch.empty(2 * B + 3, dtype=torch.int32, device=page_table.device).split_with_sizes(sizes))
+    longs = [out_slot_mapping, out_positions]
+    if longs[0] is None and longs[1] is None:
+        longs = list(torch.empty((2, n_tokens), dtype=torch.int64, device=page_table.device).unbind(0))
+    for outs, dtype, want, names in ((ints, torch.int32, sizes, ("out_seqused_k", "out_cu_seqlens_q", "out_free_count", "out_pages_taken")),
+                                     (longs, torch.int64, (n_tokens, n_tokens), ("out_slot_mapping", "out_positions"))):
+        for i, t in enumerate(outs):
+            if t is None:
+                outs[i] = torch.empty(want[i], dtype=dtype, device=page_table.device)
+            elif t.dtype != dtype or t.ndim != 1 or t.shape[0] != want[i] or not t.is_contiguous() or _require_cuda(names[i], t) != dev:
+                raise ValueError(f"{names[i]} must be a contiguous {dtype} tensor of {want[i]} elements on the page table's device")
+    seqused, cu, count, taken = ints
+    slots, positions = longs
+    _native.check(_native.load().kb200_build_ragged_step(
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], batch_idx.data_ptr(),
+        int(batch_idx.dtype == torch.int64), lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(),
+        free_pages.shape[0], free_count.data_ptr(), out_page_table.data_ptr(), out_page_table.stride(0),
+        out_page_table.shape[1], seqused.data_ptr(), cu.data_ptr(), slots.data_ptr(), positions.data_ptr(), n_tokens,
+        count.data_ptr(), taken.data_ptr(), B, int(n_pages), int(page_size), dev, _stream(dev)))
+    return RaggedStep(out_page_table, seqused, cu, slots, positions, count, taken)
+
+
+def release_rows(page_table: torch.Tensor, batch_idx: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, page_size: int, *, keep_pages: Optional[torch.Tensor] = None) -> None:
+    """Give the pages of finished requests back to ``free_pages`` (last page of a row first, as ``PageTable.erase``);
+    ``free_count`` grows, the table entries become -1.  ``keep_pages`` int32 ``[B]``: leading pages of each row that
+    stay allocated (a cached prefix).  Rows distinct; row 0 is left alone."""
+    dev = _require_cuda("page_table", page_table)
+    if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.stride(1) != 1:
+        raise ValueError("page_table must be int32 [rows, pages] contiguous in the last dimension")
+    if _require_cuda("batch_idx", batch_idx) != dev or batch_idx.ndim != 1 or not batch_idx.is_contiguous() \
+            or batch_idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError("batch_idx must be a contiguous 1-D int32/int64 tensor on the page table's device")
+    B = batch_idx.shape[0]
+    for nm, t, n in (("lengths", lengths, B), ("free_pages", free_pages, 0), ("free_count", free_count, 1)) + (
+            (("keep_pages", keep_pages, B),) if keep_pages is not None else ()):
+        if _require_cuda(nm, t) != dev or t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous():
+            raise ValueError(f"{nm} must be a contiguous int32 tensor of at least {n} elements on the page table's device")
+    if B == 0:
+        return
+    _native.check(_native.load().kb200_release_rows(
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], batch_idx.data_ptr(),
+        int(batch_idx.dtype == torch.int64), lengths.data_ptr(), keep_pages.data_ptr() if keep_pages is not None else None,
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), B, int(page_size), dev, _stream(dev)))
 
 
 def build_slot_mapping(page_table: torch.Tensor, batch_idx: torch.Tensor, positions: torch.Tensor,
@@ -433,6 +593,74 @@ def copy_pages(caches: Sequence[torch.Tensor], src_pages, dst_pages) -> None:
                                        src_t.data_ptr(), dst_t.data_ptr(), src_t.numel(), dev, _stream(dev)))
 
 
+def reorder_beam_pages(beam_table: torch.Tensor, own_table: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor,
+                       page_size: int, caches: Sequence[torch.Tensor], *, scales: Optional[Sequence[torch.Tensor]] = None,
+                       own_rows: Optional[torch.Tensor] = None) -> None:
+    """Beam ``w`` of request ``b`` goes on from beam ``parents[b, w]``: its paged state becomes the parent's, in place and
+    in one launch for all layers.
+
+    ``beam_table`` int32 ``[B * W, cols]`` is what attention reads; ``own_table`` int32 holds every beam's private pages
+    (row ``own_rows[i]``, int64, of beam ``i``; its own number without ``own_rows``), the ones new tokens are written to.
+    With ``lengths[b]`` tokens (int32) in each beam of a request, the entries of the full pages are gathered and the tokens
+    of the page being filled are copied between the beams' private pages in every pool of ``caches``
+    (``[n_pages, H_kv, P, D]``, all the same geometry; the K and V pools of every layer).  ``scales``: the
+    ``[n_pages, H_kv]`` scale arrays of int8 pools.  ``parents`` int32 / int64 ``[B, W]``, any mapping of the beams, W at most 32.
+    """
+    dev = _require_cuda("beam_table", beam_table)
+    for nm, t in (("beam_table", beam_table), ("own_table", own_table)):
+        if _require_cuda(nm, t) != dev or t.dtype != torch.int32 or t.ndim != 2 or t.stride(1) != 1:
+            raise ValueError(f"{nm} must be int32 [rows, pages], contiguous in the last dimension, on one device")
+    if _require_cuda("parents", parents) != dev or parents.ndim != 2 or not parents.is_contiguous() \
+            or parents.dtype not in (torch.int32, torch.int64):
+        raise ValueError("parents must be a contiguous int32/int64 [batch, beams] tensor on the tables' device")
+    B, W = parents.shape
+    if beam_table.shape[0] < B * W or (own_rows is None and own_table.shape[0] < B * W):
+        raise ValueError("the tables have fewer rows than there are beams")
+    if beam_table.data_ptr() == own_table.data_ptr() and B * W:
+        raise ValueError("beam_table and own_table must be different tensors")
+    if beam_table.shape[0] > 1 and beam_table.stride(0) < beam_table.shape[1]:
+        raise ValueError("rows of beam_table must not share memory")
+    if _require_cuda("lengths", lengths) != dev or lengths.dtype != torch.int32 or lengths.ndim != 1 \
+            or lengths.shape[0] < B or not lengths.is_contiguous():
+        raise ValueError("lengths must be a contiguous int32 [batch] tensor on the tables' device")
+    if own_rows is not None and (_require_cuda("own_rows", own_rows) != dev or own_rows.dtype != torch.int64 or own_rows.ndim != 1
+                                 or own_rows.shape[0] < B * W or not own_rows.is_contiguous()):
+        raise ValueError("own_rows must be a contiguous int64 tensor with one entry per beam on the tables' device")
+    n_pages, H, row_bytes, page_stride, head_stride, scale_stride = 1, 1, 1, 0, 0, 0
+    ptrs = (C.c_void_p * max(1, len(caches)))()
+    if len(caches):
+        first = caches[0]
+        if first.ndim != 4 or first.shape[2] != page_size:
+            raise ValueError("caches must have shape [n_pages, n_heads, page_size, head_dim]")
+        shape, stride, dtype, es = first.shape, first.stride(), first.dtype, first.element_size()
+        if stride[3] != 1 or stride[2] != shape[3]:
+            raise ValueError("the tokens of one page and head must be contiguous")
+        for i, c in enumerate(caches):
+            if c.shape != shape or c.stride() != stride or c.dtype != dtype:
+                raise ValueError("all pools must share shape, strides and dtype")
+            if _require_cuda(f"caches[{i}]", c) != dev:
+                raise ValueError("all pools must live on the tables' device")
+            ptrs[i] = c.data_ptr()
+        n_pages, H, row_bytes = shape[0], shape[1], shape[3] * es
+        page_stride, head_stride = stride[0] * es, stride[1] * es
+    n_scales = len(scales) if scales is not None else 0
+    sptrs = (C.c_void_p * max(1, n_scales))()
+    for i in range(n_scales):
+        s = scales[i]
+        if _require_cuda(f"scales[{i}]", s) != dev or s.dtype != torch.float32 or s.shape != (n_pages, H) or s.stride() != scales[0].stride() \
+                or s.stride(1) != 1:
+            raise ValueError("scales must be fp32 [n_pages, n_heads] arrays with equal strides on the tables' device")
+        scale_stride = s.stride(0)
+        sptrs[i] = s.data_ptr()
+    if B == 0 or W == 0:
+        return
+    _native.check(_native.load().kb200_reorder_beam_pages(
+        ptrs, len(caches), sptrs, n_scales, page_stride, head_stride, row_bytes, H, scale_stride, n_pages,
+        beam_table.data_ptr(), beam_table.stride(0), beam_table.shape[1], own_table.data_ptr(), own_table.stride(0),
+        own_table.shape[0], own_table.shape[1], own_rows.data_ptr() if own_rows is not None else None, parents.data_ptr(),
+        int(parents.dtype == torch.int64), lengths.data_ptr(), B, W, int(page_size), dev, _stream(dev)))
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
@@ -528,13 +756,14 @@ def flash_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                    out: Optional[torch.Tensor] = None,
                    return_lse: bool = False,
                    max_seqlen_q: Optional[int] = None,
-                   shared_prefix_pages: int = 0):
+                   shared_prefix_pages: int = 0,
+                   k_block_scale: Optional[torch.Tensor] = None, v_block_scale: Optional[torch.Tensor] = None):
     """Paged attention with the call surface the reference uses for ``flash_attn_fwd``
     (``kestrel/ops/attention.py:69-86``, ``kestrel/models/moondream/text.py:158-185``).
 
     ``q [B, Sq, H_q, D]`` (or ``[total_q, H_q, D]`` with ``cu_seqlens_q``), fp16/bf16;
-    ``k, v`` the ``[n_pages, P, H_kv, D]`` pool views (q's dtype, or FP8 e4m3 as
-    float8_e4m3fn / uint8); ``page_table int32 [B, >= ceil(L/P)]``; ``seqused_k int32 [B]``.
+    ``k, v`` the ``[n_pages, P, H_kv, D]`` pool views (q's dtype, FP8 e4m3 as
+    float8_e4m3fn / uint8, or int8); ``page_table int32 [B, >= ceil(L/P)]``; ``seqused_k int32 [B]``.
     ``k_scale`` / ``v_scale``: python floats (as the reference passes) or fp32 device
     tensors with ``H_kv`` entries.  ``paged_kv_non_tma`` and ``pack_gqa`` are accepted and
     ignored (hints to the reference's kernel).  Returns ``(out, lse_or_None)``.
@@ -546,6 +775,9 @@ def flash_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     ``shared_prefix_pages=n`` (extension): the caller promises that the first ``n`` page-table entries of every
     row are the same full pages (requests attached to one cached prefix, see ``PageTable.common_prefix_pages``)
     and that every query row sees all of their keys; the prefix is then read once for the whole batch.
+
+    int8 pools (extension) come with ``k_block_scale`` / ``v_block_scale``, fp32 ``[n_pages, H_kv]`` and not negative: an element is
+    ``(code + 1/2) * scale[page, head]`` (:func:`reshape_and_cache_block_int8`).
 
     Not implemented (raise ``NotImplementedError``): dense K/V (``page_table=None``),
     ``cu_seqlens_k``, any other ``mask_mod``, a non-zero right window.
@@ -604,8 +836,18 @@ def flash_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     if k.dtype != v.dtype:
         raise ValueError("k and v must share a dtype")
     fp8 = k.dtype in (torch.float8_e4m3fn, torch.uint8)
-    if not fp8 and k.dtype != q.dtype:
+    i8 = k.dtype == torch.int8
+    if not fp8 and not i8 and k.dtype != q.dtype:
         raise ValueError(f"K/V dtype {k.dtype} must equal the query dtype {q.dtype} or be FP8 e4m3")
+    if i8:
+        if k_block_scale is None or v_block_scale is None:
+            raise ValueError("int8 K/V need k_block_scale and v_block_scale")
+        for nm, t in (("k_block_scale", k_block_scale), ("v_block_scale", v_block_scale)):
+            if _require_cuda(nm, t) != dev:
+                raise ValueError(f"{nm} must live on q's device")
+        _check_block_scales(k_block_scale, v_block_scale, n_pages, Hkv)
+    elif k_block_scale is not None or v_block_scale is not None:
+        raise ValueError(f"block scales belong to int8 K/V, got {k.dtype}")
     if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.stride(1) != 1:
         raise ValueError("page_table must be int32 [batch, pages], contiguous in the last dimension")
     if page_table.shape[0] < B:
@@ -670,7 +912,10 @@ def flash_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     a.seqlen_q = Sq
     a.n_q_heads, a.n_kv_heads, a.head_dim, a.page_size = Hq, Hkv, D, P
     a.q_dtype = _TORCH_TO_DTYPE[q.dtype]
-    a.kv_dtype = _native.DTYPE_E4M3 if fp8 else _TORCH_TO_DTYPE[k.dtype]
+    a.kv_dtype = _native.DTYPE_E4M3 if fp8 else _native.DTYPE_I8 if i8 else _TORCH_TO_DTYPE[k.dtype]
+    if i8:
+        a.k_block_scale, a.v_block_scale = k_block_scale.data_ptr(), v_block_scale.data_ptr()
+        a.block_scale_page_stride = max(k_block_scale.stride(0), Hkv)   # (of a single page: any)
     a.softmax_scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D)
     a.causal = 1 if causal else 0
     a.window_left = int(window_size_left) if window_size_left is not None and window_size_left >= 0 else -1
@@ -756,6 +1001,67 @@ def sample_step_from_logits(logits: torch.Tensor, temperatures: torch.Tensor, to
     return out
 
 
+class BeamStep(NamedTuple):
+    """What :func:`beam_step_from_logits` returns."""
+
+    tokens: torch.Tensor    # int64 [B, n_out]
+    parents: torch.Tensor   # int64 [B, n_out], the beam inside the request
+    scores: torch.Tensor    # fp32 [B, n_out]
+
+
+def beam_step_from_logits(logits: torch.Tensor, scores: torch.Tensor, n_out: int, *, finished: Optional[torch.Tensor] = None,
+                          end_token: int = 0, out: Optional[BeamStep] = None) -> BeamStep:
+    """The ``n_out`` best continuations of each request over its beams and the vocabulary: candidates are
+    ``scores[b, w] + logits[b * W + w, v] - logsumexp(logits[b * W + w])``, largest first, equal ones by the lowest
+    ``w * V + v``.
+
+    ``logits`` ``[B * W, V]`` fp32 / fp16 / bf16 (a NaN counts as -inf); ``scores`` fp32 ``[B, W]``, finite or -inf (a
+    beam that does not exist yet); ``finished`` bool ``[B, W]``: such a beam has one continuation, ``end_token``, at its own
+    score.  ``n_out`` at most 64, usually ``W`` or ``2 W``.  Returns tokens, parent beams and scores, all ``[B, n_out]``
+    (``out``: written there).  Rows with nothing finite offer only candidates of -inf.
+    """
+    dev = _require_cuda("logits", logits)
+    if logits.ndim != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must have shape [batch * beams, vocab], contiguous in the vocabulary")
+    if logits.dtype not in _ROW_DTYPES:
+        raise ValueError(f"unsupported logits dtype {logits.dtype}")
+    if _require_cuda("scores", scores) != dev or scores.dtype != torch.float32 or scores.ndim != 2 or not scores.is_contiguous():
+        raise ValueError("scores must be a contiguous fp32 [batch, beams] tensor on the logits' device")
+    B, W = scores.shape
+    V, n_out = logits.shape[1], int(n_out)
+    if logits.shape[0] != B * W:
+        raise ValueError(f"logits have {logits.shape[0]} rows, scores {B} x {W}")
+    if finished is not None:
+        if _require_cuda("finished", finished) != dev or finished.dtype != torch.bool or finished.shape != scores.shape \
+                or not finished.is_contiguous():
+            raise ValueError("finished must be a contiguous bool [batch, beams] tensor on the logits' device")
+        if not 0 <= end_token < V:
+            raise ValueError("end_token must be a token of the vocabulary")
+    if n_out < 1:
+        raise ValueError("n_out must be at least 1")
+    if out is None:
+        both = torch.empty((2, B, n_out), dtype=torch.int64, device=logits.device)
+        out = BeamStep(both[0], both[1], torch.empty((B, n_out), dtype=torch.float32, device=logits.device))
+    else:
+        out = BeamStep(*out)
+        for nm, t, dt in (("tokens", out.tokens, torch.int64), ("parents", out.parents, torch.int64), ("scores", out.scores, torch.float32)):
+            if _require_cuda(nm, t) != dev or t.dtype != dt or t.shape != (B, n_out) or not t.is_contiguous():
+                raise ValueError(f"out.{nm} must be a contiguous {dt} [batch, n_out] tensor on the logits' device")
+    if B == 0:
+        return out
+    if W == 0:
+        raise ValueError("a request needs at least one beam")
+    stream = _stream(dev)
+    lib = _native.load()
+    nbytes = int(lib.kb200_beam_workspace_bytes(B, W, V, n_out, dev))
+    ws = _workspace(dev, stream, nbytes)
+    _native.check(lib.kb200_beam_step_from_logits(
+        logits.data_ptr(), _TORCH_TO_DTYPE[logits.dtype], B, W, V, logits.stride(0), scores.data_ptr(),
+        finished.data_ptr() if finished is not None else None, int(end_token), n_out, out.tokens.data_ptr(),
+        out.parents.data_ptr(), out.scores.data_ptr(), ws.data_ptr(), nbytes, dev, stream))
+    return out
+
+
 # ---------------------------------------------------------------------------
 # runtime object
 # ---------------------------------------------------------------------------
@@ -779,6 +1085,10 @@ class _CacheOps:
     build_decode_step_metadata = staticmethod(build_decode_step_metadata)
     rope_reshape_and_cache = staticmethod(rope_reshape_and_cache)
     copy_pages = staticmethod(copy_pages)
+    reshape_and_cache_block_int8 = staticmethod(reshape_and_cache_block_int8)
+    build_ragged_step = staticmethod(build_ragged_step)
+    release_rows = staticmethod(release_rows)
+    reorder_beam_pages = staticmethod(reorder_beam_pages)
 
 
 class _RotaryOps:
@@ -798,6 +1108,7 @@ class _AttentionOps:
 
 class _SamplingOps:
     sample_step_from_logits = staticmethod(sample_step_from_logits)
+    beam_step_from_logits = staticmethod(beam_step_from_logits)
 
     def __getattr__(self, item: str):
         raise NotImplementedError(f"kestrel_kernels.sampling.{item} is outside the paged-KV path")
@@ -838,5 +1149,6 @@ def install_as_kestrel_kernels() -> None:
     sys.modules["kestrel_kernels"] = me
     sampling = types.ModuleType("kestrel_kernels.sampling")
     sampling.sample_step_from_logits = sample_step_from_logits
+    sampling.beam_step_from_logits = beam_step_from_logits
     sys.modules["kestrel_kernels.sampling"] = sampling
     me.sampling = sampling

@@ -15,6 +15,8 @@ Differences, all additive:
   raise in :meth:`PagedKVCache.update`);
 * ``build_slot_mapping`` is one kernel launch on CUDA;
 * FP8 scales may be per KV head (a sequence of ``n_heads`` floats) as well as per layer;
+* ``torch.int8`` pools with one scale per page and KV head;
+* a page table that lives on the GPU and allocates there (:class:`DevicePageTable`);
 * copy-on-write of shared pages (:meth:`PageTable.cow_page`, :func:`copy_kv_pages`),
   which the reference lacks because it only allows prefix caching with ``page_size == 1``.
 """
@@ -122,6 +124,9 @@ class PagedKVCache(torch.nn.Module):
     device tensors ``k_scale_tensor`` / ``v_scale_tensor`` for the kernels; a sequence
     of ``n_heads`` floats selects per-head scales, in which case ``k_scale`` /
     ``v_scale`` are the device vectors themselves.
+
+    ``torch.int8`` pools (not in the reference) need no scales: one per page and KV head is kept in
+    ``k_block_scale`` / ``v_block_scale`` ``[n_pages, n_heads]`` and written with the codes (:meth:`update`).
     """
 
     def __init__(self, page_table, n_heads, head_dim, dtype, pool: KVMemoryPool, *,
@@ -134,7 +139,13 @@ class PagedKVCache(torch.nn.Module):
         self.register_buffer("v_cache", v_cache)
         self.page_table = page_table
         self.quantized = dtype == torch.float8_e4m3fn
+        self.block_scaled = dtype == torch.int8
         self._kv_cache_dtype = "fp8_e4m3" if self.quantized else "auto"
+        if self.block_scaled:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("int8 KV caches keep a scale per block: k_scale and v_scale do not apply")
+            for name in ("k_block_scale", "v_block_scale"):
+                self.register_buffer(name, torch.zeros((page_table.n_pages, n_heads), dtype=torch.float32, device=pool.device))
         per_head = False
         if self.quantized:
             if k_scale is None or v_scale is None:
@@ -170,6 +181,11 @@ class PagedKVCache(torch.nn.Module):
         if slots.numel() != k_rows.shape[0]:
             raise RuntimeError("PagedKVCache.update slot size mismatch")
         slots = slots.contiguous().view(-1)
+        if self.block_scaled:
+            _k.reshape_and_cache_block_int8(
+                k_rows, v_rows, self.k_cache.permute(0, 2, 1, 3), self.v_cache.permute(0, 2, 1, 3),
+                self.k_block_scale, self.v_block_scale, slots)
+            return k_val, v_val
         _k.reshape_and_cache_flash(
             k_rows, v_rows,
             self.k_cache.permute(0, 2, 1, 3), self.v_cache.permute(0, 2, 1, 3),
@@ -181,7 +197,15 @@ class PagedKVCache(torch.nn.Module):
         """Rotary embedding of ``q`` and ``k_val`` at ``input_pos`` followed by :meth:`update`, as
         one kernel launch (``kestrel/models/moondream/text.py:125`` then ``:132``).  ``q`` and
         ``k_val`` are rotated in place; the pools end up bit-identical to the two separate calls.
-        Not in the reference."""
+        int8 pools take two launches (a block's scale needs all of its rotated rows) and always rotate
+        ``k_val`` in place.  Not in the reference."""
+        if self.block_scaled:
+            if not write_k:
+                raise NotImplementedError("int8 pools: the rotated K is written back (write_k=True)")
+            if slot_mapping.shape != input_pos.shape:
+                raise ValueError("slot_mapping must match input_pos shape")
+            _k.rope_reshape_and_cache(input_pos.reshape(-1), q, k_val, None, cos_sin_cache)
+            return self.update(input_pos, k_val, v_val, slot_mapping=slot_mapping)
         if slot_mapping.shape != input_pos.shape:
             raise ValueError("slot_mapping must match input_pos shape")
         slots = slot_mapping.to(device=k_val.device, dtype=torch.int64).contiguous().view(-1)
@@ -253,14 +277,82 @@ def allocate_paged_kv_layers(*, layer_specs: Sequence[PagedKVLayerSpec | None], 
     return tuple(layers)
 
 
-def copy_kv_pages(layers: Iterable[PagedKVCache | None], src_pages, dst_pages) -> None:
-    """Run the pending copy-on-write copies on the K and V pools of every layer in one launch."""
-    pools = []
+def _pools_and_scales(layers: Iterable[PagedKVCache | None]) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
+    """K and V pools of the layers, and the scale arrays of those that are int8."""
+    pools, scales = [], []
     for layer in layers:
         if layer is not None:
-            pools.append(layer.k_cache)
-            pools.append(layer.v_cache)
+            pools += [layer.k_cache, layer.v_cache]
+            if getattr(layer, "block_scaled", False):
+                scales += [layer.k_block_scale, layer.v_block_scale]
+    return pools, scales
+
+
+def copy_kv_pages(layers: Iterable[PagedKVCache | None], src_pages, dst_pages) -> None:
+    """Run the pending copy-on-write copies on the K and V pools of every layer in one launch (and, for int8
+    layers, on their scales)."""
+    pools, scales = _pools_and_scales(layers)
     _k.copy_pages(pools, src_pages, dst_pages)
+    if scales and scales[0].shape[1] % 4 == 0:   # (the page copy moves multiples of 16 bytes)
+        _k.copy_pages(scales, src_pages, dst_pages)
+    elif scales:
+        src = torch.as_tensor(src_pages, dtype=torch.int64, device=scales[0].device)
+        dst = torch.as_tensor(dst_pages, dtype=torch.int64, device=scales[0].device)
+        for s in scales:
+            s[dst] = s[src]
+
+
+def reorder_beams(layers: Iterable[PagedKVCache | None], beam_table: torch.Tensor, own_table: torch.Tensor,
+                  parents: torch.Tensor, lengths: torch.Tensor, *, own_rows: Optional[torch.Tensor] = None) -> None:
+    """Beam ``w`` of each request goes on from beam ``parents[b, w]`` in every layer, in one launch: see
+    :func:`kestrel_b200.kernels.reorder_beam_pages`.  ``own_table`` is the table new tokens are written through (the
+    ``page_table`` of a :class:`PageTable` whose rows ``own_rows`` belong to the beams), ``beam_table`` the one attention reads."""
+    layers = [layer for layer in layers if layer is not None]
+    if not layers:
+        raise ValueError("reorder_beams needs at least one layer")
+    pools, scales = _pools_and_scales(layers)
+    _k.reorder_beam_pages(beam_table, own_table, parents, lengths, layers[0].k_cache.shape[2], pools,
+                          scales=scales or None, own_rows=own_rows)
+
+
+class DevicePageTable:
+    """A page table that lives on the GPU and hands out its pages there, from request lengths.
+
+    ``page_table [max_batch_size, pages_per_row]`` int32, ``free_pages`` and ``free_count``: the pool's free list in device
+    memory.  :meth:`step` does for a whole ragged step (decode rows and prompt chunks alike) what
+    ``PageTable.reserve``, ``commit_block_table``, ``populate_paged_kv_metadata`` and ``build_slot_mapping`` do row by row on the
+    host, in one launch and capturable; :meth:`release` is ``PageTable.erase``.  Row 0 and page 0 are reserved for padding,
+    as in :class:`PageTable`, and pages leave the list in the same order.  Usable wherever a :class:`PagedKVCache`
+    wants a page table.
+    """
+
+    def __init__(self, n_pages: int, page_size: int, max_batch_size: int, device: torch.device | str = "cuda", *,
+                 pages_per_row: int | None = None):
+        if n_pages < 1 or page_size < 1 or max_batch_size < 1:
+            raise ValueError("n_pages, page_size and max_batch_size must be positive")
+        self.n_pages, self.page_size, self.max_batch_size = n_pages, page_size, max_batch_size
+        self.device = resolve_device(device)
+        cols = n_pages if pages_per_row is None else int(pages_per_row)
+        if cols < 1:
+            raise ValueError("pages_per_row must be positive")
+        self.page_table = torch.full((max_batch_size, cols), -1, dtype=torch.int32, device=self.device)
+        self.page_table[0] = 0
+        self.free_pages = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=self.device)
+        self.free_count = torch.full((1,), n_pages - 1, dtype=torch.int32, device=self.device)
+
+    def step(self, batch_idx: torch.Tensor, lengths: torch.Tensor, new_tokens: torch.Tensor, n_tokens: int, *,
+             out_page_table: torch.Tensor, out_seqused_k: torch.Tensor | None = None, **outs: torch.Tensor) -> _k.RaggedStep:
+        """Allocate and map one step: entry ``i`` holds ``lengths[i]`` tokens and appends ``new_tokens[i]``.  See
+        :func:`kestrel_b200.kernels.build_ragged_step`; ``free_count`` is advanced in place, ``out_seqused_k=lengths``
+        advances the lengths too."""
+        return _k.build_ragged_step(self.page_table, batch_idx, lengths, new_tokens, self.free_pages, self.free_count,
+                                    self.page_size, n_pages=self.n_pages, n_tokens=n_tokens, out_page_table=out_page_table,
+                                    out_seqused_k=out_seqused_k, out_free_count=self.free_count, **outs)
+
+    def release(self, batch_idx: torch.Tensor, lengths: torch.Tensor, keep_pages: torch.Tensor | None = None) -> None:
+        """The rows' pages (but for their first ``keep_pages``) go back to the free list."""
+        _k.release_rows(self.page_table, batch_idx, lengths, self.free_pages, self.free_count, self.page_size,
+                        keep_pages=keep_pages)
 
 
 class PageTable:
