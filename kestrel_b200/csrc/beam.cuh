@@ -1,31 +1,42 @@
 // Beam search on the paged cache: selection over beams and vocabulary, and the reordering of the beams' pages.
 //
 // Selection.  cand(w, v) = score_w + x_wv - log sum_u exp x_wu; the K largest over the W * V candidates of a request, equal
-// ones by the lowest w * V + v.  Inside a row the order is the logits' own, so a row's K best are found on the logits
-// (exactly, in one pass that also gathers maximum and sum); only the few survivors are put on the common scale, in 64 bits.
-//   beam_slice_kernel  one CTA per slice of a row, the slice in registers.  The K-th largest of the 256 threads' own
-//                      maxima is a threshold that the slice's K best cannot lie below, and what lies at or above it
-//                      belongs to K threads: at most K * EPT elements to rank, K and a few as a rule.
+// ones by the lowest w * V + v.  Inside a row the order is the logits' own, so a row's K best are found on the logits,
+// exactly; only the few survivors are put on the common scale, in 64 bits.
+//   beam_slice_kernel  one CTA per slice of a row, one pass: every thread keeps the maximum of its elements and the sum of
+//                      their exponentials.  The K-th largest of 64 groups' maxima is a threshold that the slice's K best
+//                      cannot lie below; only the threads whose own maximum reaches it (K and a few) have their
+//                      elements read again, out of L2, and what reaches it there is ranked.
 //   beam_merge_kernel  one CTA per request: log-sum-exps of its rows, then the same threshold over their candidates.
 // HBM-bound: the logits are read once.  Nothing depends on the order in which threads arrive.
+//
+// Sums.  exp x = 2^(x L' - e) 2^e with L' the fp32 log2(e) and e = ceil(max x L') a whole number, so that raising the maximum
+// scales a sum by a power of two, exactly; 32 terms at a time in fp32, 64 bits from there on.  L' is off by 1.3e-8
+// relatively; for the terms that matter x is close to e / L', and log sum exp x = e / L' + log sum 2^(x L' - e) takes that out.
 #pragma once
 
+#include "paged_prefill.cuh"   // packed fp32 arithmetic
 #include "sampling.cuh"
 
 namespace kb200 {
 
 constexpr int kBeamThreads = 256;
+constexpr int kBeamGroups = 64;        // of 4 neighbouring threads; at least kBeamMaxOut
 constexpr int kBeamMaxOut = 64;
 constexpr int kBeamMaxBeams = 64;
-constexpr int kBeamMergeThreads = 512;
-constexpr int kBeamMergeKeep = 1024;   // survivors that the merge ranks at once; more (never seen) take the slow way
+constexpr int kBeamKeep = 1024;        // survivors that are ranked at once; more (rows made for it) take the slow way
+constexpr int kBeamCtasPerSm = 4;      // slices that are cut per SM when rows alone are too few
+constexpr float kBeamLog2e = 1.4426950408889634f;
+static_assert(kBeamGroups >= kBeamMaxOut, "the K-th largest group maximum must exist");
+
+struct BeamSum { double s; float e; float pad; };   // s * 2^e; e = -inf: nothing
 
 struct BeamParams {
   const char* logits;
   const float* scores;
   const uint8_t* finished;     // or nullptr
   unsigned long long* part;    // [rows][slices][K] keys: ordered logit << 32 | ~index
-  float2* part_ml;             // [rows][slices] maximum, sum of exp(x - maximum)
+  BeamSum* part_sum;           // [rows][slices]
   int64_t* out_tokens;
   int64_t* out_parents;
   float* out_scores;
@@ -33,7 +44,7 @@ struct BeamParams {
   int batch, beams, n_out, n_slices, slice, vec_ok;
 };
 
-// floats ordered as unsigned integers, NaN below everything but 0
+// floats ordered as unsigned integers
 __device__ __forceinline__ uint32_t order_f32(float x) {
   const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
@@ -46,112 +57,255 @@ __device__ __forceinline__ unsigned long long order_f64(double x) {
 __device__ __forceinline__ double unorder_f64(unsigned long long o) {
   return __longlong_as_double((long long)((o >> 63) ? o & ~(1ull << 63) : ~o));
 }
+// 2^(a - b) for whole numbers a <= b (0 below 2^-1000)
+__device__ __forceinline__ double pow2_diff(float a, float b) {
+  const float d = a - b;
+  return d > -1000.f ? __hiloint2double((1023 + (int)d) << 20, 0) : 0.0;
+}
+__device__ __forceinline__ float beam_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// (-0 and 0 are equal, NaN counts as -inf)
+__device__ __forceinline__ float beam_value(float x) { return x == x ? x + 0.f : -INFINITY; }
+__device__ __forceinline__ unsigned long long beam_key(float x, uint32_t i) { return ((unsigned long long)order_f32(x) << 32) | (uint32_t)~i; }
 
-// EPT elements per thread, in vectors of 16 bytes
-template <typename LT, int EPT>
-__global__ void __launch_bounds__(kBeamThreads) beam_slice_kernel(const BeamParams p) {
-  constexpr int N = SampleVec<LT>::N;
-  constexpr int NV = EPT / N;
-  __shared__ __align__(16) unsigned long long keys[kBeamThreads];
-  __shared__ unsigned long long kept[kBeamMaxOut * EPT];
-  __shared__ float red_m[kBeamThreads / 32];
-  __shared__ double red_s[kBeamThreads / 32];
+template <typename LT>
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(const BeamParams p) {
+  constexpr int N = SampleVec<LT>::N;      // elements of a 16-byte vector
+  constexpr int U = 4;                     // vectors in flight
+  constexpr int NW = kBeamThreads / 32;
+  __shared__ __align__(16) unsigned long long group_key[kBeamGroups];
+  __shared__ unsigned long long kept[kBeamKeep];
+  __shared__ BeamSum red[NW];
   __shared__ unsigned long long threshold;
-  __shared__ int n_kept;
+  __shared__ int picked[kBeamThreads];     // threads whose elements are read again
+  __shared__ int n_picked, n_kept;
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int64_t r = blockIdx.y;
   const int sl = blockIdx.x, K = p.n_out;
-  const LT* row = reinterpret_cast<const LT*>(p.logits) + r * p.row_stride;
-  const int64_t lo = (int64_t)sl * p.slice, hi = min(lo + p.slice, p.vocab);
-
-  // the slice: vector j of this thread starts at lo + (j * threads + tid) * N; what lies past the end is -inf
-  float x[EPT];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int64_t i = lo + ((int64_t)j * kBeamThreads + tid) * N;
-    if (p.vec_ok && i + N <= hi) {
+  const int64_t lo = (int64_t)sl * p.slice;
+  const LT* row = reinterpret_cast<const LT*>(p.logits) + r * p.row_stride + lo;
+  const int len = (int)(min(lo + p.slice, p.vocab) - lo);   // (elements are counted from the slice's start from here on)
+  const bool vec = p.vec_ok != 0;
+  // vector v of thread t starts at (v * threads + t) * N; what lies past the end is -inf
+  const int nv = (len + kBeamThreads * N - 1) / (kBeamThreads * N);
+  auto load = [&](int i, float (&x)[N]) {
+    if (vec && i + N <= len) {
       const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + i));
       const LT* e = reinterpret_cast<const LT*>(&raw);
 #pragma unroll
-      for (int k = 0; k < N; ++k) x[j * N + k] = logit_to_float<LT>(e[k]);
+      for (int k = 0; k < N; ++k) x[k] = logit_to_float<LT>(e[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < N; ++k) x[j * N + k] = i + k < hi ? logit_to_float<LT>(__ldg(row + i + k)) : -INFINITY;
+      for (int k = 0; k < N; ++k) x[k] = -INFINITY;
+      if (i < len) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (i + k < len) x[k] = logit_to_float<LT>(__ldg(row + i + k));
+      }
+    }
+  };
+
+  // One pass.  Of the maximum only the batch is kept that it was met in: its place is looked up at the end (some lane of a
+  // warp meets a new maximum in nearly every batch, and a search there would cost more than everything else).
+  float m = -INFINITY, e2 = -INFINITY;
+  int best_v = 0;
+  double sum = 0.0;
+  // x[] in [.., top]: the running maximum and the sum of exponentials take a batch in
+  auto take = [&](int v0, float top, const float (&x)[U * N]) {
+    if (top > m) {
+      m = top;
+      best_v = v0;
+      const float e_new = ceilf(m * kBeamLog2e);
+      if (e_new > e2) {
+        sum *= pow2_diff(e2, e_new);
+        e2 = e_new;
+      }
+    }
+    if (m > -INFINITY) {
+      const uint64_t l2 = pack_f32x2(kBeamLog2e, kBeamLog2e), ne = pack_f32x2(-e2, -e2);
+      uint64_t a0 = 0ull, a1 = 0ull;   // (bit pattern of 0.f, 0.f)
+#pragma unroll
+      for (int i = 0; i < U * N; i += 4) {
+        float y0, y1, y2, y3;
+        unpack_f32x2(fma_f32x2(pack_f32x2(x[i], x[i + 1]), l2, ne), y0, y1);
+        unpack_f32x2(fma_f32x2(pack_f32x2(x[i + 2], x[i + 3]), l2, ne), y2, y3);
+        a0 = add_f32x2(a0, pack_f32x2(beam_ex2(y0), beam_ex2(y1)));
+        a1 = add_f32x2(a1, pack_f32x2(beam_ex2(y2), beam_ex2(y3)));
+      }
+      float s0, s1;
+      unpack_f32x2(add_f32x2(a0, a1), s0, s1);
+      sum += (double)(s0 + s1);
+    }
+  };
+  const int nv_full = vec ? len / (kBeamThreads * N) / U * U : 0;   // vectors that every thread has in whole, in batches
+  const LT* mine_at = row + tid * N;
+  auto stream = [&](bool clean) {
+    uint4 raw[U], next[U];   // the next batch is on its way while this one is summed up
+    if (nv_full > 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = __ldg(reinterpret_cast<const uint4*>(mine_at + u * (kBeamThreads * N)));
+    }
+    for (int v0 = 0; v0 < nv_full; v0 += U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      if (v0 + U < nv_full) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          next[u] = __ldg(reinterpret_cast<const uint4*>(mine_at + (v0 + U + u) * (kBeamThreads * N)));
+      }
+      float x[U * N], tops[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const LT* e = reinterpret_cast<const LT*>(&raw[u]);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float f = logit_to_float<LT>(e[k]);
+          x[u * N + k] = clean ? beam_value(f) : f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        tops[u] = fmaxf(x[u * N], x[u * N + 1]);
+#pragma unroll
+        for (int k = 2; k < N; k += 2) tops[u] = max3(tops[u], x[u * N + k], x[u * N + k + 1]);
+      }
+      take(v0, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), x);
+    }
+    for (int v0 = nv_full; v0 < nv; v0 += U) {
+      float x[U * N], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float y[N];
+        load(((v0 + u) * kBeamThreads + tid) * N, y);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          x[u * N + k] = clean ? beam_value(y[k]) : y[k];
+          top = fmaxf(top, x[u * N + k]);
+        }
+      }
+      take(v0, top, x);
+    }
+  };
+  stream(false);
+  if (!(sum == sum)) {   // a NaN or an infinity among the logits
+    m = e2 = -INFINITY;
+    best_v = 0;
+    sum = 0.0;
+    stream(true);
+  }
+  int best_i = tid * N;   // (a thread without a number above -inf: its first element)
+  const bool any = best_i < len;
+  if (m > -INFINITY) {
+    bool found = false;
+    for (int v = best_v; !found && v < nv; ++v) {
+      const int i = (v * kBeamThreads + tid) * N;
+      float x[N];
+      load(i, x);
+#pragma unroll
+      for (int k = N - 1; k >= 0; --k)
+        if (x[k] == m) { found = true; best_i = i + k; }   // (the lowest one stays)
     }
   }
-  auto index_of = [&](int e) { return (uint32_t)(lo + ((int64_t)(e / N) * kBeamThreads + tid) * N + e % N); };
-  // this thread's best: largest value, then lowest index (indices ascend with e)
-  float best = -INFINITY;
-  int best_e = 0;
-  if (tid == 0) n_kept = 0;
+  const uint32_t first = (uint32_t)lo;
+
+  // sums and maxima across the CTA
+  const unsigned long long mine = any ? beam_key(m + 0.f, first + best_i) : 0ull;
+  {
+    float e = e2;
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) {
-    x[e] = x[e] == x[e] ? x[e] + 0.f : -INFINITY;   // NaN: never chosen before a number; -0 and 0 are equal
-    if (x[e] > best) { best = x[e]; best_e = e; }
+    for (int d = 16; d > 0; d >>= 1) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, d));
+    double s = e2 > -INFINITY ? sum * pow2_diff(e2, e) : 0.0;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (lane == 0) red[wid] = BeamSum{s, e, 0.f};
+    unsigned long long g = mine;
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      const unsigned long long o = __shfl_xor_sync(0xffffffffu, g, d);
+      g = o > g ? o : g;
+    }
+    if ((tid & 3) == 0) group_key[tid >> 2] = g;
   }
-  const uint32_t first_i = index_of(0);
-  const bool any = first_i < hi;
-  keys[tid] = any ? ((unsigned long long)order_f32(best) << 32) | (uint32_t)~index_of(best_e) : 0ull;
-  float m = best;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (lane == 0) red_m[wid] = m;
+  if (tid == 0) { threshold = 0ull; n_picked = 0; n_kept = 0; }   // (fewer groups with elements than K: everything is kept)
   __syncthreads();
-  m = red_m[0];
-#pragma unroll
-  for (int w = 1; w < kBeamThreads / 32; ++w) m = fmaxf(m, red_m[w]);
-
-  // sum of exp(x - m): fp32 inside a thread (at most EPT terms), 64 bits across
-  float s = 0.f;
-  if (m > -INFINITY) {
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) s += exp2f((x[e] - m) * 1.4426950408889634f);
-  }
-  double sd = s;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, d);
-  if (lane == 0) red_s[wid] = sd;
-
-  // rank of this thread's maximum among the threads' (keys are distinct, but for the zeros of empty threads)
-  const unsigned long long mine = keys[tid];
-  int above = 0;
-  const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(keys);
+  if (tid < kBeamGroups) {
+    const unsigned long long g = group_key[tid];
+    int above = 0;
+    const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(group_key);
 #pragma unroll 8
-  for (int i = 0; i < kBeamThreads / 2; ++i) {
-    const ulonglong2 v = k2[i];
-    above += (v.x > mine) + (v.y > mine);
-  }
-  if (tid == 0) threshold = 0ull;   // (fewer threads with elements than K: everything is kept)
-  __syncthreads();
-  if (mine != 0ull && above == K - 1) threshold = mine;
-  if (tid == 0) {
-    double t = 0.0;
-#pragma unroll
-    for (int w = 0; w < kBeamThreads / 32; ++w) t += red_s[w];
-    p.part_ml[r * p.n_slices + sl] = make_float2(m, (float)t);
+    for (int i = 0; i < kBeamGroups / 2; ++i) {
+      const ulonglong2 o = k2[i];
+      above += (o.x > g) + (o.y > g);
+    }
+    if (g != 0ull && above == K - 1) threshold = g;
+  } else if (wid == NW - 1 && lane == 0) {
+    BeamSum t = red[0];
+    for (int w = 1; w < NW; ++w) t.e = fmaxf(t.e, red[w].e);
+    t.s = 0.0;
+    for (int w = 0; w < NW; ++w) t.s += red[w].e > -INFINITY ? red[w].s * pow2_diff(red[w].e, t.e) : 0.0;
+    p.part_sum[r * p.n_slices + sl] = t;
   }
   __syncthreads();
   const unsigned long long thr = threshold;
-  if (mine != 0ull && mine >= thr) {
+  if (mine != 0ull && mine >= thr) picked[atomicAdd(&n_picked, 1)] = tid;   // (any order: the survivors are ranked)
+  __syncthreads();
+  const int np = n_picked;
+  const float thr_x = thr ? unorder_f32((uint32_t)(thr >> 32)) : -INFINITY;
+  for (int j = wid; j < np; j += NW) {       // a warp per thread whose elements are read again
+    const int t = picked[j];
+    for (int v = lane; v < nv; v += 32) {
+      const int i = (v * kBeamThreads + t) * N;
+      float x[N];
+      load(i, x);
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      const uint32_t i = index_of(e);
-      const unsigned long long key = ((unsigned long long)order_f32(x[e]) << 32) | (uint32_t)~i;
-      if (i < hi && key >= thr) kept[atomicAdd(&n_kept, 1)] = key;   // (their order is settled by the ranks below)
+      for (int k = 0; k < N; ++k) {
+        if (x[k] < thr_x || i + k >= len) continue;   // (nearly all; NaN goes on)
+        const unsigned long long key = beam_key(beam_value(x[k]), first + i + k);
+        if (key >= thr) {
+          const int at = atomicAdd(&n_kept, 1);
+          if (at < kBeamKeep) kept[at] = key;
+        }
+      }
     }
   }
   __syncthreads();
   const int n = n_kept;
   unsigned long long* out = p.part + (r * p.n_slices + sl) * K;
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const unsigned long long key = kept[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += kept[j] > key;
-    if (rank < K) out[rank] = key;
+  if (n <= kBeamKeep) {
+    for (int i = tid; i < n; i += kBeamThreads) {
+      const unsigned long long key = kept[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += kept[j] > key;
+      if (rank < K) out[rank] = key;
+    }
+    for (int i = n + tid; i < K; i += kBeamThreads) out[i] = 0ull;   // a slice shorter than K
+    return;
   }
-  for (int i = n + tid; i < K; i += kBeamThreads) out[i] = 0ull;   // a slice shorter than K
+  // too many to rank: K rounds, each the best element behind the last one
+  unsigned long long last = ~0ull;
+  for (int rank = 0; rank < K; ++rank) {
+    unsigned long long top = 0ull;
+    for (int v = 0; v < nv; ++v) {
+      const int i = (v * kBeamThreads + tid) * N;
+      float x[N];
+      load(i, x);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const unsigned long long key = beam_key(beam_value(x[k]), first + i + k);
+        if (i + k < len && key < last && key > top) top = key;
+      }
+    }
+    __syncthreads();
+    kept[tid] = top;
+    __syncthreads();
+    for (int d = kBeamThreads / 2; d > 0; d >>= 1) {
+      if (tid < d && kept[tid + d] > kept[tid]) kept[tid] = kept[tid + d];
+      __syncthreads();
+    }
+    last = kept[0];
+    if (tid == 0) out[rank] = last;
+  }
 }
 
 // A candidate on the common scale.  Larger is better; equal values by the lower flat index.
@@ -161,12 +315,12 @@ struct BeamCand {
   __device__ __forceinline__ bool before(const BeamCand& o) const { return v > o.v || (v == o.v && i < o.i); }
 };
 
-__global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const BeamParams p) {
-  constexpr int NT = kBeamMergeThreads;
+__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamParams p) {
+  constexpr int NT = kBeamThreads;
   __shared__ double base[kBeamMaxBeams];      // score - log-sum-exp; the score itself for a finished beam
   __shared__ int kind[kBeamMaxBeams];         // 0 a live row, 1 finished, 2 nothing to offer
-  __shared__ unsigned long long top_v[NT], top_i[NT];
-  __shared__ unsigned long long kept_v[kBeamMergeKeep], kept_i[kBeamMergeKeep];
+  __shared__ unsigned long long group_v[kBeamGroups], group_i[kBeamGroups];
+  __shared__ unsigned long long kept_v[kBeamKeep], kept_i[kBeamKeep];
   __shared__ unsigned long long thr_v, thr_i;
   __shared__ int n_kept;
   pdl_wait();
@@ -177,19 +331,22 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
   const int64_t V = p.vocab;
   // log-sum-exps: a warp per row
   for (int w = wid; w < W; w += NT / 32) {
-    const float2* ml = p.part_ml + (b * W + w) * S;
-    float m = -INFINITY;
-    for (int s = lane; s < S; s += 32) m = fmaxf(m, ml[s].x);
+    const BeamSum* ps = p.part_sum + (b * W + w) * S;
+    float e = -INFINITY;
+    for (int s = lane; s < S; s += 32) e = fmaxf(e, ps[s].e);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int d = 16; d > 0; d >>= 1) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, d));
     double sum = 0.0;
-    for (int s = lane; s < S; s += 32) sum += ml[s].x > -INFINITY ? (double)ml[s].y * exp((double)ml[s].x - (double)m) : 0.0;
+    for (int s = lane; s < S; s += 32) {
+      const BeamSum t = ps[s];
+      if (t.e > -INFINITY) sum += t.s * pow2_diff(t.e, e);
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) {
       const float score = p.scores[b * W + w];
       const bool fin = p.finished && p.finished[b * W + w] != 0;
-      const double lse = (double)m + log(sum);
+      const double lse = (double)e / (double)kBeamLog2e + log(sum);
       const bool finite = fabsf(score) < INFINITY && (fin || (lse - lse == 0.0));
       kind[w] = !finite ? 2 : fin ? 1 : 0;
       base[w] = (fin ? (double)score : (double)score - lse) + 0.0;
@@ -200,10 +357,10 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
 
   // candidate c of the request: rank k of slice s of row w.  Neighbouring threads take different rows and slices of one
   // rank, so that the good ones are spread over the threads.
-  const int n_cand = W * S * K;
+  const int WS = W * S, n_cand = WS * K;
   const unsigned long long kMinusInf = order_f64(-INFINITY);
   auto candidate = [&](int c) -> BeamCand {
-    const int k = c / (W * S), ws = c - k * (W * S), w = ws / S, s = ws - w * S;
+    const int k = c / WS, ws = c - k * WS, w = ws / S, s = ws - w * S;
     BeamCand r{0ull, ~0ull};
     const int kd = kind[w];
     if (kd == 0) {
@@ -234,32 +391,40 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
     p.out_scores[at] = (float)unorder_f64(c.v);
   };
 
+  const bool one = n_cand <= NT;   // a thread has one candidate at most: it stays in registers
   BeamCand best{0ull, ~0ull};
   for (int c = tid; c < n_cand; c += NT) {
     const BeamCand v = candidate(c);
     if (v.v != 0ull && v.before(best)) best = v;
   }
-  top_v[tid] = best.v;
-  top_i[tid] = best.i;
+  BeamCand g = best;
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    const BeamCand o{__shfl_xor_sync(0xffffffffu, g.v, d), __shfl_xor_sync(0xffffffffu, g.i, d)};
+    if (o.before(g)) g = o;
+  }
+  if ((tid & 3) == 0) { group_v[tid >> 2] = g.v; group_i[tid >> 2] = g.i; }
   __syncthreads();
-  if (best.v != 0ull) {
+  if (tid < kBeamGroups) {
+    const BeamCand mine{group_v[tid], group_i[tid]};
     int above = 0;
-    for (int i = 0; i < NT; ++i) above += BeamCand{top_v[i], top_i[i]}.before(best);
-    if (above == K - 1) { thr_v = best.v; thr_i = best.i; }
+#pragma unroll 8
+    for (int i = 0; i < kBeamGroups; ++i) above += BeamCand{group_v[i], group_i[i]}.before(mine);
+    if (mine.v != 0ull && above == K - 1) { thr_v = mine.v; thr_i = mine.i; }
   }
   __syncthreads();
   const BeamCand thr{thr_v, thr_i};
   if (best.v != 0ull && !thr.before(best)) {
     for (int c = tid; c < n_cand; c += NT) {
-      const BeamCand v = candidate(c);
+      const BeamCand v = one ? best : candidate(c);
       if (v.v == 0ull || thr.before(v)) continue;
       const int at = atomicAdd(&n_kept, 1);
-      if (at < kBeamMergeKeep) { kept_v[at] = v.v; kept_i[at] = v.i; }
+      if (at < kBeamKeep) { kept_v[at] = v.v; kept_i[at] = v.i; }
     }
   }
   __syncthreads();
   const int n = n_kept;
-  if (n <= kBeamMergeKeep) {
+  if (n <= kBeamKeep) {
     for (int i = tid; i < n; i += NT) {
       const BeamCand c{kept_v[i], kept_i[i]};
       int rank = 0;
@@ -277,37 +442,37 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
       if (v.v != 0ull && last.before(v) && v.before(mine)) mine = v;
     }
     __syncthreads();
-    top_v[tid] = mine.v;
-    top_i[tid] = mine.i;
+    kept_v[tid] = mine.v;
+    kept_i[tid] = mine.i;
     __syncthreads();
     for (int d = NT / 2; d > 0; d >>= 1) {
       if (tid < d) {
-        const BeamCand o{top_v[tid + d], top_i[tid + d]};
-        if (o.before(BeamCand{top_v[tid], top_i[tid]})) { top_v[tid] = o.v; top_i[tid] = o.i; }
+        const BeamCand o{kept_v[tid + d], kept_i[tid + d]};
+        if (o.before(BeamCand{kept_v[tid], kept_i[tid]})) { kept_v[tid] = o.v; kept_i[tid] = o.i; }
       }
       __syncthreads();
     }
-    last = BeamCand{top_v[0], top_i[0]};
+    last = BeamCand{kept_v[0], kept_i[0]};
     if (tid == 0) write(rank, last);
   }
 }
 
-// Elements per thread of the slice kernel: 32 (one wave of loads in flight, few partial lists), 8 when the rows
-// alone would not give every SM a CTA.
+// Slices per row: enough CTAs to fill every SM, none below 2048 elements (a vector of 16-bit logits per thread).
 inline int beam_slice_len(int64_t rows, int64_t vocab, int sms) {
-  const int64_t big = 32 * kBeamThreads;
-  return rows * ((vocab + big - 1) / big) >= sms ? (int)big : 8 * kBeamThreads;
+  int64_t n = (kBeamCtasPerSm * (int64_t)sms + rows - 1) / rows;
+  if (n > (vocab + 2047) / 2048) n = (vocab + 2047) / 2048;
+  if (n < 1) n = 1;
+  return (int)(((vocab + n - 1) / n + 7) / 8 * 8);
 }
 inline uint64_t beam_workspace_need(int64_t batch, int64_t beams, int64_t vocab, int64_t n_out, int sms) {
   const int64_t rows = batch * beams, slice = beam_slice_len(rows, vocab, sms), S = (vocab + slice - 1) / slice;
-  return (uint64_t)(rows * S * n_out * 8 + rows * S * 8);
+  return (uint64_t)(rows * S * n_out * 8 + rows * S * sizeof(BeamSum));
 }
 
 template <typename LT>
 inline int launch_beam_slices(const BeamParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)p.n_slices, (unsigned)(p.batch * p.beams));
-  if (p.slice == 32 * kBeamThreads) KB200_CUDA_OK(launch_kernel(beam_slice_kernel<LT, 32>, grid, dim3(kBeamThreads), 0, stream, p));
-  else KB200_CUDA_OK(launch_kernel(beam_slice_kernel<LT, 8>, grid, dim3(kBeamThreads), 0, stream, p));
+  KB200_CUDA_OK(launch_kernel(beam_slice_kernel<LT>, grid, dim3(kBeamThreads), 0, stream, p));
   return KB200_OK;
 }
 
@@ -453,15 +618,15 @@ inline int launch_beam_step(const void* logits, int logits_dtype, int64_t batch,
   p.n_out = (int)n_out;
   p.slice = beam_slice_len(batch * beams, vocab, sms);
   p.n_slices = (int)((vocab + p.slice - 1) / p.slice);
-  p.part = static_cast<unsigned long long*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part + batch * beams * p.n_slices * n_out);
+  p.part_sum = static_cast<BeamSum*>(workspace);
+  p.part = reinterpret_cast<unsigned long long*>(p.part_sum + batch * beams * p.n_slices);
   p.vec_ok = ((reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (row_stride * es) % 16 == 0) ? 1 : 0;
   int rc;
   if (logits_dtype == KB200_DTYPE_F32) rc = launch_beam_slices<float>(p, stream);
   else if (logits_dtype == KB200_DTYPE_F16) rc = launch_beam_slices<__half>(p, stream);
   else rc = launch_beam_slices<__nv_bfloat16>(p, stream);
   if (rc) return rc;
-  KB200_CUDA_OK(launch_kernel(beam_merge_kernel, dim3((unsigned)batch), dim3(kBeamMergeThreads), 0, stream, p));
+  KB200_CUDA_OK(launch_kernel(beam_merge_kernel, dim3((unsigned)batch), dim3(kBeamThreads), 0, stream, p));
   return KB200_OK;
 }
 
