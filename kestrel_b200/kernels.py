@@ -39,6 +39,8 @@ _ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _require_cuda(name: str, t: torch.Tensor) -> int:
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        return t.get_device()
     if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
         dev = getattr(t, "device", type(t).__name__)
         raise RuntimeError(
@@ -48,7 +50,7 @@ def _require_cuda(name: str, t: torch.Tensor) -> int:
 
 
 def _stream(device_index: int) -> int:
-    return torch.cuda.current_stream(device_index).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device_index)   # (what torch.cuda.current_stream wraps, without the wrapper object)
 
 
 def _cache_view_geometry(name: str, cache: torch.Tensor) -> tuple[int, int, int, int, int, int, int]:
@@ -227,7 +229,7 @@ def build_ragged_step(page_table: torch.Tensor, batch_idx: torch.Tensor, lengths
     B, n_tokens = batch_idx.shape[0], int(n_tokens)
     for nm, t, n in (("lengths", lengths, B), ("new_tokens", new_tokens, B), ("free_pages", free_pages, 0),
                      ("free_count", free_count, 1)):
-        if _require_cuda(nm, t) != dev or t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] < n or not t.is_contiguous():
+        if _require_cuda(nm, t) != dev or t.dtype != torch.int32 or t.ndim != 1 or t.numel() < n or not t.is_contiguous():
             raise ValueError(f"{nm} must be a contiguous int32 tensor of at least {n} elements on the page table's device")
     if _require_cuda("batch_idx", batch_idx) != dev or batch_idx.ndim != 1 or not batch_idx.is_contiguous() \
             or batch_idx.dtype not in (torch.int32, torch.int64):
@@ -239,22 +241,20 @@ def build_ragged_step(page_table: torch.Tensor, batch_idx: torch.Tensor, lengths
         raise ValueError("out_page_table has fewer rows than the batch")
     if n_tokens < 0:
         raise ValueError("n_tokens must not be negative")
-    ints = [out_seqused_k, out_cu_seqlens_q, out_free_count, out_pages_taken]
-    sizes = (B, B + 1, 1, 1)
-    if not any(t is not None for t in ints):   # (one buffer: a step of a few requests is bound by its host side)
-        ints = list(torch.empty(2 * B + 3, dtype=torch.int32, device=page_table.device).split_with_sizes(sizes))
-    longs = [out_slot_mapping, out_positions]
-    if longs[0] is None and longs[1] is None:
-        longs = list(torch.empty((2, n_tokens), dtype=torch.int64, device=page_table.device).unbind(0))
-    for outs, dtype, want, names in ((ints, torch.int32, sizes, ("out_seqused_k", "out_cu_seqlens_q", "out_free_count", "out_pages_taken")),
-                                     (longs, torch.int64, (n_tokens, n_tokens), ("out_slot_mapping", "out_positions"))):
-        for i, t in enumerate(outs):
-            if t is None:
-                outs[i] = torch.empty(want[i], dtype=dtype, device=page_table.device)
-            elif t.dtype != dtype or t.ndim != 1 or t.shape[0] != want[i] or not t.is_contiguous() or _require_cuda(names[i], t) != dev:
-                raise ValueError(f"{names[i]} must be a contiguous {dtype} tensor of {want[i]} elements on the page table's device")
-    seqused, cu, count, taken = ints
-    slots, positions = longs
+
+    def out(nm: str, t: Optional[torch.Tensor], n: int, dtype: torch.dtype) -> torch.Tensor:
+        if t is None:
+            return torch.empty(n, dtype=dtype, device=page_table.device)
+        if t.dtype != dtype or t.ndim != 1 or t.numel() != n or not t.is_contiguous() or _require_cuda(nm, t) != dev:
+            raise ValueError(f"{nm} must be a contiguous {dtype} tensor of {n} elements on the page table's device")
+        return t
+
+    seqused = out("out_seqused_k", out_seqused_k, B, torch.int32)
+    cu = out("out_cu_seqlens_q", out_cu_seqlens_q, B + 1, torch.int32)
+    count = out("out_free_count", out_free_count, 1, torch.int32)
+    taken = out("out_pages_taken", out_pages_taken, 1, torch.int32)
+    slots = out("out_slot_mapping", out_slot_mapping, n_tokens, torch.int64)
+    positions = out("out_positions", out_positions, n_tokens, torch.int64)
     _native.check(_native.load().kb200_build_ragged_step(
         page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], batch_idx.data_ptr(),
         int(batch_idx.dtype == torch.int64), lengths.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(),
@@ -627,31 +627,31 @@ def reorder_beam_pages(beam_table: torch.Tensor, own_table: torch.Tensor, parent
                                  or own_rows.shape[0] < B * W or not own_rows.is_contiguous()):
         raise ValueError("own_rows must be a contiguous int64 tensor with one entry per beam on the tables' device")
     n_pages, H, row_bytes, page_stride, head_stride, scale_stride = 1, 1, 1, 0, 0, 0
-    ptrs = (C.c_void_p * max(1, len(caches)))()
     if len(caches):
         first = caches[0]
-        if first.ndim != 4 or first.shape[2] != page_size:
+        shape, dtype, es = first.shape, first.dtype, first.element_size()
+        if len(shape) != 4 or shape[2] != page_size:
             raise ValueError("caches must have shape [n_pages, n_heads, page_size, head_dim]")
-        shape, stride, dtype, es = first.shape, first.stride(), first.dtype, first.element_size()
+        stride = first.stride()
         if stride[3] != 1 or stride[2] != shape[3]:
             raise ValueError("the tokens of one page and head must be contiguous")
-        for i, c in enumerate(caches):
-            if c.shape != shape or c.stride() != stride or c.dtype != dtype:
+        dense = first.is_contiguous()
+        for i, c in enumerate(caches):   # (a few dozen pools: the checks are most of what the call costs the host)
+            if c.shape != shape or c.dtype != dtype or not (dense and c.is_contiguous() or c.stride() == stride):
                 raise ValueError("all pools must share shape, strides and dtype")
-            if _require_cuda(f"caches[{i}]", c) != dev:
+            if _require_cuda("caches[i]", c) != dev:
                 raise ValueError("all pools must live on the tables' device")
-            ptrs[i] = c.data_ptr()
         n_pages, H, row_bytes = shape[0], shape[1], shape[3] * es
         page_stride, head_stride = stride[0] * es, stride[1] * es
     n_scales = len(scales) if scales is not None else 0
-    sptrs = (C.c_void_p * max(1, n_scales))()
-    for i in range(n_scales):
-        s = scales[i]
-        if _require_cuda(f"scales[{i}]", s) != dev or s.dtype != torch.float32 or s.shape != (n_pages, H) or s.stride() != scales[0].stride() \
-                or s.stride(1) != 1:
-            raise ValueError("scales must be fp32 [n_pages, n_heads] arrays with equal strides on the tables' device")
-        scale_stride = s.stride(0)
-        sptrs[i] = s.data_ptr()
+    if n_scales:
+        want, s_stride = torch.Size((n_pages, H)), scales[0].stride()
+        for s in scales:
+            if s.shape != want or s.dtype != torch.float32 or s.stride() != s_stride or _require_cuda("scales[i]", s) != dev or s_stride[1] != 1:
+                raise ValueError("scales must be fp32 [n_pages, n_heads] arrays with equal strides on the tables' device")
+        scale_stride = s_stride[0]
+    ptrs = (C.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
+    sptrs = (C.c_void_p * max(1, n_scales))(*[s.data_ptr() for s in scales or ()])
     if B == 0 or W == 0:
         return
     _native.check(_native.load().kb200_reorder_beam_pages(

@@ -61,6 +61,8 @@ def test_ties_go_to_the_lowest_index():
     for V in (3, 40, 9000):
         for x in (torch.zeros(2, V), torch.zeros(2, V).index_fill_(1, torch.tensor([1]), -0.0)):
             _select(x, torch.zeros(1, 2), min(6, 2 * V))
+    # 64 of 64 equal rows: over a thousand elements of a slice and candidates of the request reach the thresholds
+    _select(torch.zeros(64, 20000), torch.zeros(1, 64), 64)
 
 
 def test_first_step_and_dead_rows():
