@@ -346,8 +346,8 @@ KB200_API int kb200_sample_step_from_logits(
  *   key_scales, value_scales  device fp32 [n_pages, n_kv_heads], page stride given in elements
  *   slot_mapping      device int64 [num_tokens]; negative slots are skipped.  The tokens of one block are
  *                     neighbours in the mapping, as any layout by sequence leaves them; a block whose tokens come in
- *                     two separate runs of one call is left with undefined codes (nothing else is touched).  Of
- *                     equal slots in a run the last one counts.
+ *                     two separate runs of one call (a skipped token between them separates them, too) is left with
+ *                     undefined codes (nothing else is touched).  Of equal slots in a run the last one counts.
  */
 KB200_API int kb200_append_block_int8(
     const void* key, const void* value, int64_t key_token_stride, int64_t value_token_stride, void* key_cache,

@@ -146,7 +146,8 @@ def reshape_and_cache_block_int8(key: torch.Tensor, value: torch.Tensor, key_cac
     block's rows, the code ``floor(x / s)``, so that an element is off by at most ``s / 2``.  A block whose first
     token is written starts anew; a later, larger row raises the scale and shifts the codes already there.  The bytes do not
     depend on how a block's tokens are split over calls.  The tokens of one block have to be neighbours in
-    ``slot_mapping``; of equal neighbouring slots the last one counts.  A NaN is stored as code 0, an infinity saturates
+    ``slot_mapping``, with no other and no skipped token between them (the block's codes are undefined otherwise); of equal
+    neighbouring slots the last one counts.  A NaN is stored as code 0, an infinity saturates
     (``STATUS_NOT_FINITE``).
     """
     dev = _require_cuda("key", key)

@@ -30,6 +30,17 @@ def quantize_block(rows: torch.Tensor) -> tuple[torch.Tensor, float]:
     return code.to(torch.int8), s
 
 
+def quantize_blocks(rows: torch.Tensor, live: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The same for finite ``rows [B, P, D]`` of many blocks at once; ``live [B, P]``: the rows that exist (codes of the
+    others are 0)."""
+    x = torch.where(live.unsqueeze(-1), rows.double(), torch.zeros((), dtype=torch.float64, device=rows.device))
+    amax = x.abs().amax((1, 2))
+    _, e = torch.frexp(amax)
+    s = torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), (e - 7).clamp(min=-126)), torch.zeros_like(amax))
+    code = torch.where(s.view(-1, 1, 1) > 0, torch.floor(x / s.view(-1, 1, 1).clamp(min=2.0 ** -126)), torch.zeros_like(x))
+    return code.to(torch.int8), s
+
+
 def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """``[n_pages, H, P, D]`` codes and ``[n_pages, H]`` scales -> float64 values."""
     return (codes.double() + 0.5) * scales.double()[:, :, None, None]

@@ -94,6 +94,70 @@ def test_bytes_do_not_depend_on_the_split(dtype, P, H, D):
             assert torch.equal(cache[page], before[kv][page].cpu()) and torch.equal(scale[page], before[2 + kv][page].cpu())
 
 
+@pytest.mark.parametrize("dtype,P,H,D", [(torch.bfloat16, 64, 8, 128), (torch.float16, 16, 8, 64), (torch.float32, 128, 8, 64),
+                                         (torch.bfloat16, 256, 8, 128), (torch.bfloat16, 24, 16, 32), (torch.float32, 4, 8, 128)])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_many_tokens(dtype, P, H, D, aligned):
+    """Prompt chunks in numbers that give every warp a window of its own: two calls per sequence, the second one starting
+    inside a page; a NaN, an infinity, a skipped token and equal slots among them."""
+    _clear_status()
+    g = torch.Generator(device=DEV).manual_seed(P + D)
+    lengths = [1 + (i * 977) % 1500 for i in range(28)]
+    pages = [-(-n // P) for n in lengths]
+    n_pages = sum(pages) + 2
+    perm = torch.randperm(n_pages, generator=g, device=DEV)
+    table = torch.zeros(len(lengths), max(pages), dtype=torch.int64, device=DEV)
+    at = 0
+    for b, c in enumerate(pages):
+        table[b, :c] = perm[at:at + c]
+        at += c
+    seq = torch.cat([torch.full((n,), b, device=DEV) for b, n in enumerate(lengths)])
+    pos = torch.cat([torch.arange(n, device=DEV) for n in lengths])
+    T = len(pos)
+    extra = 0 if aligned else 1        # rows off the 16-byte boundary
+    k, v = (torch.randn(T * H * D + 1, generator=g, device=DEV).to(dtype)[extra:extra + T * H * D].view(T, H, D) for _ in range(2))
+    slots = table[seq, pos // P] * P + pos % P
+    kc, vc, ks, vs = _pools(n_pages, H, P, D)
+    first = pos < torch.tensor([n * 2 // 3 for n in lengths], device=DEV)[seq]
+    for part in (first, ~first):
+        i = torch.nonzero(part).view(-1)
+        a, b = k[i], v[i]
+        if not aligned:
+            a, b = (torch.cat([x.reshape(-1)[:1], x.reshape(-1)])[1:].view(x.shape) for x in (a, b))
+        _append(a, b, kc, vc, ks, vs, slots[i])
+    block = table[seq, pos // P]
+    live = torch.zeros(n_pages, P, dtype=torch.bool, device=DEV)
+    live[block, pos % P] = True
+    for x, cache, scale in ((k, kc, ks), (v, vc, vs)):
+        for h in range(H):
+            rows = torch.zeros(n_pages, P, D, dtype=dtype, device=DEV)
+            rows[block, pos % P] = x[:, h]
+            code, s = O.quantize_blocks(rows, live)
+            used = live.any(1)
+            assert torch.equal(scale[used, h].double(), s[used]), h
+            assert torch.equal(cache[:, h][live], code[live]), h
+    assert _native.device_status(0)[0] == 0
+    # the same once more in one call, with what does not belong there
+    k2 = k.clone()
+    long = lengths.index(max(lengths))
+    at = int(torch.nonzero(seq == long)[0])
+    k2[at + 3, 0, :3] = torch.tensor([math.nan, math.inf, -math.inf], dtype=dtype, device=DEV)
+    slots2 = slots.clone()
+    slots2[at + min(P, 3) - 1 + P * 2] = -1 if P > 4 else slots2[at + min(P, 3) - 1 + P * 2]
+    if P > 8:
+        slots2[at + P + 5] = slots2[at + P + 4]       # the later row counts
+    _append(k2, v, kc, vc, ks, vs, slots2)
+    assert _native.device_status(0)[0] == _native.STATUS_NOT_FINITE
+    for c in range(2):
+        page = int(table[long, c])
+        toks = [t for t in range(at + c * P, at + min(lengths[long], (c + 1) * P)) if int(slots2[t]) >= 0]
+        code, s = O.quantize_block(k2[toks, 0].cpu())
+        assert float(ks[page, 0]) == s
+        for j, t in enumerate(toks):
+            if int(slots2[t]) not in slots2[t + 1:at + (c + 1) * P].tolist():
+                assert torch.equal(kc[page, 0, int(slots2[t]) % P].cpu(), code[j]), (c, j)
+
+
 def test_strides_alignment_negative_and_equal_slots():
     """Rows that are slices of a fused projection, rows off the 16-byte boundary, skipped tokens, equal slots in a run."""
     g = torch.Generator().manual_seed(3)
