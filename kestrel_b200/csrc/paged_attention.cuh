@@ -278,17 +278,75 @@ __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t x, uint32_t& lo, uint32
       : "=r"(lo), "=r"(hi)
       : "r"(x));
 }
-// Four int8 codes (one 32-bit word) -> code + 1/2 as f16, bytes 0 and 2 in `lo`, bytes 1 and 3 in `hi`; exact.  In
-// [512, 1024) an f16 has steps of 1/2: the code's eight bits, its sign flipped, go to mantissa bits 1-8 and a one to bit 0,
-// which makes 512 + (code + 128) + 1/2.
+__device__ __forceinline__ float bf16_bits_to_float(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
+// Four int8 codes (one 32-bit word) as f16 pairs, bytes 0 and 2 in `lo`, bytes 1 and 3 in `hi`.  A code with its sign flipped is
+// u = code + 128 in [0, 256), and the 16 bits 00uu are the f16 (subnormal) number u 2^-24: a mask makes an operand.
+// K is used as that; q . u differs from q . (code + 1/2) by 127.5 sum(q), which the accumulators start with.  For V one
+// fma gives (code + 1/2) 2^-9, exactly (a sum over thousands of keys must not carry such an offset).
+__device__ __forceinline__ void i8x4_to_u16x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  lo = (x & 0x00ff00ffu) ^ 0x00800080u;
+  hi = ((x >> 8) & 0x00ff00ffu) ^ 0x00800080u;
+}
 __device__ __forceinline__ void i8x4_to_f16x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
-  const uint32_t a = ((x << 1) & 0x01fe01feu) ^ 0x61016101u, b = ((x >> 7) & 0x01fe01feu) ^ 0x61016101u;
-  const __half2 c = __float2half2_rn(640.f);
-  const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&a), c), rb = __hsub2(*reinterpret_cast<const __half2*>(&b), c);
+  uint32_t a, b;
+  i8x4_to_u16x4(x, a, b);
+  const __half2 s = __float2half2_rn(32768.f), o = __float2half2_rn(-255.f / 1024.f);
+  const __half2 ra = __hfma2(*reinterpret_cast<const __half2*>(&a), s, o), rb = __hfma2(*reinterpret_cast<const __half2*>(&b), s, o);
   lo = *reinterpret_cast<const uint32_t*>(&ra);
   hi = *reinterpret_cast<const uint32_t*>(&rb);
 }
-// the pairs that i8x4_to_f16x4 makes, for four consecutive 16-bit elements in two words
+constexpr float kI8KeyUnit = 16777216.f;                        // a product with K in units of 2^-24
+constexpr float kI8KeyOffset = -127.5f / 16777216.f;            // what its accumulator starts with, per unit of sum(q)
+constexpr float kI8ValUnit = 512.f;                             // V in units of 2^-9
+// The 8- and 16-row kernels multiply the codes as they are: mma.sync m16n8k32 on int8 runs at the instruction rate of m16n8k16 on
+// f16 (measured), so a product with q as a 16-bit number in two bytes costs what the f16 product costs, and K needs no
+// conversion at all (the three ALU operations per word of the mask above were a seventh of a decode call).
+// q_d = delta n_d with delta = max|q| / 32512 per row, n = 256 hi + lo; off by at most delta / 2, 2^-16 of the row's largest.
+// sum(n c) <= 2^22 per byte plane: accumulators that start at the bits of 1.5 * 2^23 come out as floats.
+constexpr float kI8Magic = 12582912.f;
+constexpr int kI8MagicBits = 0x4b400000;
+__device__ __forceinline__ void imma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four consecutive q (16-bit pairs w0, w1) as floats
+__device__ __forceinline__ void q4_to_floats(uint32_t w0, uint32_t w1, bool bf16, float (&f)[4]) {
+  if (bf16) {
+    f[0] = bf16_bits_to_float(w0 & 0xffffu); f[1] = bf16_bits_to_float(w0 >> 16);
+    f[2] = bf16_bits_to_float(w1 & 0xffffu); f[3] = bf16_bits_to_float(w1 >> 16);
+  } else {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w0)), b = __half22float2(*reinterpret_cast<const __half2*>(&w1));
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  }
+}
+__device__ __forceinline__ float q4_max(uint32_t w0, uint32_t w1, bool bf16) {
+  float f[4];
+  q4_to_floats(w0, w1, bf16, f);
+  return fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+}
+// the high and low bytes of n = rint(q inv), four to a word; returns their sum
+__device__ __forceinline__ int q4_to_bytes(uint32_t w0, uint32_t w1, bool bf16, float inv, uint32_t& hi, uint32_t& lo) {
+  float f[4];
+  q4_to_floats(w0, w1, bf16, f);
+  int n[4], h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    n[i] = __float2int_rn(f[i] * inv);
+    h[i] = (n[i] + 128) >> 8;   // n - 256 h in [-128, 127]
+  }
+  hi = __byte_perm(__byte_perm(h[0], h[1], 0x0040), __byte_perm(h[2], h[3], 0x0040), 0x5410);
+  lo = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+  return (n[0] + n[1]) + (n[2] + n[3]);
+}
+constexpr float kI8QueryMax = 32512.f;   // 256 * 127: the high byte stays in [-127, 127]
+// sum of the two halves of an f16 pair
+__device__ __forceinline__ float f16x2_sum(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f.x + f.y;
+}
+// the pairs that i8x4_to_u16x4 makes, for four consecutive 16-bit elements in two words
 __device__ __forceinline__ void pair_02_13(uint32_t& w0, uint32_t& w1) {
   const uint32_t e = __byte_perm(w0, w1, 0x5410), o = __byte_perm(w0, w1, 0x7632);
   w0 = e;
@@ -298,6 +356,10 @@ __device__ __forceinline__ void pair_02_13(uint32_t& w0, uint32_t& w1) {
 template <int KPL>
 struct TileScales {
   float k[KPL], v[KPL];
+  __device__ __forceinline__ void apply_unit(float unit) {   // (once per tile, when the loads have arrived)
+#pragma unroll
+    for (int u = 0; u < KPL; ++u) k[u] *= unit;
+  }
   // of key base + off of the tile; base: a constant of an unrolled loop, off < 8
   __device__ __forceinline__ float key(int base, int off) const { return __shfl_sync(0xffffffffu, k[base >> 5], (base & 31) + off); }
   __device__ __forceinline__ float val(int base, int off) const { return __shfl_sync(0xffffffffu, v[base >> 5], (base & 31) + off); }
@@ -323,7 +385,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&v);
   }
 }
-__device__ __forceinline__ float bf16_bits_to_float(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 
 // ---------------------------------------------------------------------------
 // Plan: per-sequence tile/segment counts and their exclusive prefix sums.
@@ -650,9 +711,13 @@ struct TileProducer {
       int page;
       if constexpr (GATHER) page = key < pc.L ? pt_row[key >> p_shift] : -1;
       else page = __shfl_sync(0xffffffffu, pg, (i >> box_shift) << 1);   // (rows of at most 128 bytes: K and V, a box each)
-      const bool ok = key < pc.L && (unsigned)page < (unsigned long long)p.n_pages;
-      ts.k[u] = ok ? p.kbs[page * p.bs_ps + h] : 0.f;
-      ts.v[u] = ok ? p.vbs[page * p.bs_ps + h] : 0.f;
+      const bool ok = key < pc.L && (unsigned)page < (unsigned)p.n_pages;   // (page indices and int8 pools' sizes: 31 bits)
+      const int64_t at = (int64_t)page * p.bs_ps + h;
+      ts.k[u] = ts.v[u] = 0.f;
+      if (ok) {
+        ts.k[u] = p.kbs[at];
+        ts.v[u] = p.vbs[at];
+      }
     }
   }
 };
@@ -728,6 +793,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
   float sl2 = 0.f, vscale = 1.f;
   [[maybe_unused]] float vref = 0.f, vinv = 0.f;   // (I8) largest V scale seen, and what a V scale is multiplied by
+  [[maybe_unused]] float si0 = 0.f, si1 = 0.f, dq0 = 0.f, dq1 = 0.f;   // (I8) rows g and g + 8: sum(n) / 2 and delta of q = delta n
+  [[maybe_unused]] const bool uni16 = p.page_size >= 16;   // (I8) 16 neighbouring keys share their scales
   int lim0 = 0, lim1 = 0, row0 = 0, row1 = 0, h = 0;
   bool valid0 = false, valid1 = false;
   bool fresh = true;
@@ -780,14 +847,45 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           const int d = 16 * ch + 4 * c4;
           uint2 a = valid0 ? *reinterpret_cast<const uint2*>(q0 + 2 * d) : make_uint2(0u, 0u);
           uint2 b = valid1 ? *reinterpret_cast<const uint2*>(q1 + 2 * d) : make_uint2(0u, 0u);
-          if (p.q_is_bf16) {
+          if (!I8 && p.q_is_bf16) {
             a.x = pack2<false>(bf16_bits_to_float(a.x & 0xffffu), bf16_bits_to_float(a.x >> 16));
             a.y = pack2<false>(bf16_bits_to_float(a.y & 0xffffu), bf16_bits_to_float(a.y >> 16));
             b.x = pack2<false>(bf16_bits_to_float(b.x & 0xffffu), bf16_bits_to_float(b.x >> 16));
             b.y = pack2<false>(bf16_bits_to_float(b.y & 0xffffu), bf16_bits_to_float(b.y >> 16));
           }
-          if constexpr (I8) { pair_02_13(a.x, a.y); pair_02_13(b.x, b.y); }
           qf[ch][0] = a.x; qf[ch][1] = b.x; qf[ch][2] = a.y; qf[ch][3] = b.y;
+        }
+        if constexpr (I8) {   // as byte planes: qf[ch] = { high bytes of row g, of row g + 8, low bytes of row g, of row g + 8 }
+          const bool qbf = p.q_is_bf16 != 0;
+          float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+          for (int ch = 0; ch < NQF; ++ch) {
+            t0 = fmaxf(t0, q4_max(qf[ch][0], qf[ch][2], qbf));
+            t1 = fmaxf(t1, q4_max(qf[ch][1], qf[ch][3], qbf));
+          }
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+          }
+          const float v0 = t0 > 0.f ? kI8QueryMax / t0 : 0.f, v1 = t1 > 0.f ? kI8QueryMax / t1 : 0.f;
+          int n0 = 0, n1 = 0;
+#pragma unroll
+          for (int ch = 0; ch < NQF; ++ch) {
+            uint32_t h0, l0_, h1, l1_;
+            n0 += q4_to_bytes(qf[ch][0], qf[ch][2], qbf, v0, h0, l0_);
+            n1 += q4_to_bytes(qf[ch][1], qf[ch][3], qbf, v1, h1, l1_);
+            qf[ch][0] = h0; qf[ch][1] = h1; qf[ch][2] = l0_; qf[ch][3] = l1_;
+          }
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) {
+            n0 += __shfl_xor_sync(0xffffffffu, n0, d);
+            n1 += __shfl_xor_sync(0xffffffffu, n1, d);
+          }
+          si0 = 0.5f * (float)n0;
+          si1 = 0.5f * (float)n1;
+          dq0 = t0 * (1.f / kI8QueryMax);
+          dq1 = t1 * (1.f / kI8QueryMax);
         }
       }
     }
@@ -831,6 +929,36 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           mma16816<BF16>(s[n], qf[2 * q4 + 1], b2, b3);
         }
       }
+    } else if constexpr (I8) {
+      // the bytes of a K fragment are the int8 operand; one accumulator per byte plane of q; s = delta k_scale (256 h + l + sum(n) / 2)
+      float ka = 0.f, kb = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT8; ++n) {
+        const int r = n * 8 + (lane & 7);
+        int sh[4] = {kI8MagicBits, kI8MagicBits, kI8MagicBits, kI8MagicBits}, sl[4] = {kI8MagicBits, kI8MagicBits, kI8MagicBits, kI8MagicBits};
+#pragma unroll
+        for (int q4 = 0; q4 < HD / 64; ++q4) {
+          uint32_t x[4];   // key r, d = 64 q4 + 16 i + 4c ..
+          ldsm_x4(x[0], x[1], x[2], x[3], kbase + (uint32_t)r * RB + ((uint32_t)((q4 * 4 + (lane >> 3)) ^ swz<RB>(r)) << 4));
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const int ch = q4 * 4 + i;
+            imma16832(sh, qf[ch][0], qf[ch][1], qf[ch + 1][0], qf[ch + 1][1], x[i], x[i + 1]);
+            imma16832(sl, qf[ch][2], qf[ch][3], qf[ch + 1][2], qf[ch + 1][3], x[i], x[i + 1]);
+          }
+        }
+        if (!uni16) {
+          ka = sc_cur.key(n * 8, 2 * c4);
+          kb = sc_cur.key(n * 8, 2 * c4 + 1);
+        } else if (n % 2 == 0) {
+          ka = kb = sc_cur.key(n * 8, 0);
+        }
+        auto join = [&](int i, float half) { return fmaf(__int_as_float(sh[i]) - kI8Magic, 256.f, __int_as_float(sl[i]) - kI8Magic) + half; };
+        s[n][0] = join(0, si0) * (ka * dq0);
+        s[n][1] = join(1, si0) * (kb * dq0);
+        s[n][2] = join(2, si1) * (ka * dq1);
+        s[n][3] = join(3, si1) * (kb * dq1);
+      }
     } else {
 #pragma unroll
       for (int n = 0; n < NT8; ++n) {
@@ -844,19 +972,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t b0, b1;
-            if constexpr (I8) i8x4_to_f16x4(x[i], b0, b1);
-            else e4m3x4_to_f16x4(x[i], b0, b1);
+            e4m3x4_to_f16x4(x[i], b0, b1);
             mma16816<false>(s[n], qf[q4 * 4 + i], b0, b1);
           }
         }
-      }
-    }
-
-    if constexpr (I8) {
-#pragma unroll
-      for (int n = 0; n < NT8; ++n) {
-        const float ka = sc_cur.key(n * 8, 2 * c4), kb = sc_cur.key(n * 8, 2 * c4 + 1);
-        s[n][0] *= ka; s[n][1] *= kb; s[n][2] *= ka; s[n][3] *= kb;
       }
     }
 
@@ -911,12 +1030,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         vref = vmax;
         vinv = kVScaleUp / vmax;
-        vscale = vmax * (1.f / kVScaleUp);
+        vscale = vmax * (kI8ValUnit / kVScaleUp);
       }
     }
     const float ms0 = (m0 == -INFINITY) ? 0.f : m0 * sl2;
     const float ms1 = (m1 == -INFINITY) ? 0.f : m1 * sl2;
     uint32_t pf[NKS][4];
+    [[maybe_unused]] float va = 0.f, vb = 0.f;
 #pragma unroll
     for (int n = 0; n < NT8; ++n) {
       const float p0 = ex2(fmaf(s[n][0], sl2, -ms0));
@@ -926,7 +1046,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       l0 += p0 + p1;
       l1 += p2 + p3;
       if constexpr (I8) {
-        const float va = sc_cur.val(n * 8, 2 * c4) * vinv, vb = sc_cur.val(n * 8, 2 * c4 + 1) * vinv;
+        if (!uni16 || n % 2 == 0) va = vb = sc_cur.val(n * 8, uni16 ? 0 : 2 * c4) * vinv;
+        if (!uni16) vb = sc_cur.val(n * 8, 2 * c4 + 1) * vinv;
         pf[n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0 * va, p1 * vb);
         pf[n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2 * va, p3 * vb);
       } else {
@@ -1217,6 +1338,8 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;   // running max / partial sum of query rows 2c and 2c+1
   float sl2 = 0.f, vscale = 1.f;
   [[maybe_unused]] float vref = 0.f, vinv = 0.f;   // (I8) largest V scale seen, and what a V scale is multiplied by
+  [[maybe_unused]] float si0 = 0.f, si1 = 0.f, dq0 = 0.f, dq1 = 0.f;   // (I8) rows 2c, 2c + 1: sum(n) / 2 and delta of q = delta n
+  [[maybe_unused]] const bool uni16 = p.page_size >= 16;   // (I8) 16 neighbouring keys share their scales
   int lim0 = 0, lim1 = 0, h = 0, mb = 0;
   bool fresh = true;
   long long piece_start = r0;
@@ -1270,13 +1393,36 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             d -= q_slice * p.real_hd;
           }
           uint2 a = mine ? *reinterpret_cast<const uint2*>(qrow + 2 * d) : make_uint2(0u, 0u);
-          if (p.q_is_bf16) {
+          if (!I8 && p.q_is_bf16) {
             a.x = pack2<false>(bf16_bits_to_float(a.x & 0xffffu), bf16_bits_to_float(a.x >> 16));
             a.y = pack2<false>(bf16_bits_to_float(a.y & 0xffffu), bf16_bits_to_float(a.y >> 16));
           }
-          if constexpr (I8) pair_02_13(a.x, a.y);
           qb[ch][0] = a.x;
           qb[ch][1] = a.y;
+        }
+        if constexpr (I8) {   // row g8 as byte planes: qb[ch][0] the high ones of d = 16ch + 4c .., qb[ch][1] the low ones
+          const bool qbf = p.q_is_bf16 != 0;
+          float top = 0.f;
+#pragma unroll
+          for (int ch = 0; ch < NDT; ++ch) top = fmaxf(top, q4_max(qb[ch][0], qb[ch][1], qbf));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float inv = top > 0.f ? kI8QueryMax / top : 0.f;
+          int ns = 0;
+#pragma unroll
+          for (int ch = 0; ch < NDT; ++ch) {
+            uint32_t hi, lo;
+            ns += q4_to_bytes(qb[ch][0], qb[ch][1], qbf, inv, hi, lo);
+            qb[ch][0] = hi;
+            qb[ch][1] = lo;
+          }
+          ns += __shfl_xor_sync(0xffffffffu, ns, 1);
+          ns += __shfl_xor_sync(0xffffffffu, ns, 2);
+          const float half = 0.5f * (float)ns, delta = top * (1.f / kI8QueryMax);
+          si0 = __shfl_sync(0xffffffffu, half, 8 * c4);
+          si1 = __shfl_sync(0xffffffffu, half, 8 * c4 + 4);
+          dq0 = __shfl_sync(0xffffffffu, delta, 8 * c4);
+          dq1 = __shfl_sync(0xffffffffu, delta, 8 * c4 + 4);
         }
       }
     }
@@ -1301,7 +1447,7 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     const uint32_t vbase = kbase + T::KV_TILE_BYTES;
     const int key0 = (cc.tile0 + cc.t) * TILE_N;
 
-    auto widen = [](uint32_t x, uint32_t& e, uint32_t& o_) {
+    auto widen_v = [](uint32_t x, uint32_t& e, uint32_t& o_) {
       if constexpr (I8) i8x4_to_f16x4(x, e, o_);
       else e4m3x4_to_f16x4(x, e, o_);
     };
@@ -1327,6 +1473,40 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           else mma16816r<BF16>(s[mt], a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
         }
       }
+    } else if constexpr (I8) {
+      // the bytes of a K fragment are the int8 operand; one accumulator per byte plane of q
+      int sh[NMT][4], sl[NMT][4];
+#pragma unroll
+      for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sh[mt][i] = sl[mt][i] = kI8MagicBits;
+#pragma unroll
+      for (int cp = 0; cp < NDT / 2; ++cp) {
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt) {
+          uint32_t x0, x1, x2, x3;  // (keys lo, ch) (keys hi, ch) (keys lo, ch+1) (keys hi, ch+1)
+          ldsm_x4(x0, x1, x2, x3, kbase + kv8_off(mt * 16 + k_row, 2 * cp + k_chunk));
+          imma16832(sh[mt], x0, x1, x2, x3, qb[2 * cp][0], qb[2 * cp + 1][0]);
+          imma16832(sl[mt], x0, x1, x2, x3, qb[2 * cp][1], qb[2 * cp + 1][1]);
+        }
+      }
+      // s = delta k_scale (256 h + l + sum(n) / 2)
+      auto join = [](int h, int l) { return fmaf(__int_as_float(h) - kI8Magic, 256.f, __int_as_float(l) - kI8Magic); };
+      if (uni16) {
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt) {
+          const float ka = sc_cur.key(mt * 16, 0), f0 = ka * dq0, f1 = ka * dq1, o0 = f0 * si0, o1 = f1 * si1;
+          s[mt][0] = fmaf(join(sh[mt][0], sl[mt][0]), f0, o0); s[mt][1] = fmaf(join(sh[mt][1], sl[mt][1]), f1, o1);
+          s[mt][2] = fmaf(join(sh[mt][2], sl[mt][2]), f0, o0); s[mt][3] = fmaf(join(sh[mt][3], sl[mt][3]), f1, o1);
+        }
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt) {
+          const float ka = sc_cur.key(mt * 16, g8), kb = sc_cur.key(mt * 16 + 8, g8);
+          s[mt][0] = (join(sh[mt][0], sl[mt][0]) + si0) * (ka * dq0); s[mt][1] = (join(sh[mt][1], sl[mt][1]) + si1) * (ka * dq1);
+          s[mt][2] = (join(sh[mt][2], sl[mt][2]) + si0) * (kb * dq0); s[mt][3] = (join(sh[mt][3], sl[mt][3]) + si1) * (kb * dq1);
+        }
+      }
     } else {
 #pragma unroll
       for (int cp = 0; cp < NDT / 2; ++cp) {
@@ -1338,28 +1518,20 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           uint32_t x0, x1, x2, x3;  // (keys lo, ch) (keys hi, ch) (keys lo, ch+1) (keys hi, ch+1)
           ldsm_x4(x0, x1, x2, x3, addr);
           uint32_t a0, a1, a2, a3;
-          widen(x0, a0, a2);
-          widen(x1, a1, a3);
+          e4m3x4_to_f16x4(x0, a0, a2);
+          e4m3x4_to_f16x4(x1, a1, a3);
           mma16816r<false>(s[mt], a0, a1, a2, a3, qb[2 * cp][0], qb[2 * cp][1]);
-          widen(x2, a0, a2);
-          widen(x3, a1, a3);
+          e4m3x4_to_f16x4(x2, a0, a2);
+          e4m3x4_to_f16x4(x3, a1, a3);
           mma16816r<false>(s2[mt], a0, a1, a2, a3, qb[2 * cp + 1][0], qb[2 * cp + 1][1]);
         }
       }
     }
 #pragma unroll
-    for (int mt = 0; mt < NMT; ++mt) {
+    for (int mt = 0; mt < NMT && !I8; ++mt) {
       s[mt][0] += s2[mt][0]; s[mt][1] += s2[mt][1]; s[mt][2] += s2[mt][2]; s[mt][3] += s2[mt][3];
     }
     // s[mt] = { (key 16mt+g, q 2c), (key 16mt+g, q 2c+1), (key 16mt+g+8, q 2c), (key 16mt+g+8, q 2c+1) }
-
-    if constexpr (I8) {
-#pragma unroll
-      for (int mt = 0; mt < NMT; ++mt) {
-        const float ka = sc_cur.key(mt * 16, g8), kb = sc_cur.key(mt * 16 + 8, g8);
-        s[mt][0] *= ka; s[mt][1] *= ka; s[mt][2] *= kb; s[mt][3] *= kb;
-      }
-    }
 
     // ---- mask (only tiles that touch a boundary)
     const int key_last = key0 + TILE_N - 1;
@@ -1413,12 +1585,25 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         }
         vref = vmax;
         vinv = kVScaleUp / vmax;
-        vscale = vmax * (1.f / kVScaleUp);
+        vscale = vmax * (kI8ValUnit / kVScaleUp);
       }
     }
     const float ms0 = (m0 == -INFINITY) ? 0.f : m0 * sl2;
     const float ms1 = (m1 == -INFINITY) ? 0.f : m1 * sl2;
     uint32_t pb[NMT][2];  // P^T B fragments per 16-key block
+    [[maybe_unused]] float va[NMT], vb[NMT];   // (I8) what the weights of keys 16mt + g8 and 16mt + 8 + g8 are multiplied by
+    if constexpr (I8) {
+      if (uni16) {
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt) va[mt] = vb[mt] = sc_cur.val(mt * 16, 0) * vinv;
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt) {
+          va[mt] = sc_cur.val(mt * 16, g8) * vinv;
+          vb[mt] = sc_cur.val(mt * 16 + 8, g8) * vinv;
+        }
+      }
+    }
 #pragma unroll
     for (int mt = 0; mt < NMT; ++mt) {
       const float p0 = ex2(fmaf(s[mt][0], sl2, -ms0));
@@ -1427,10 +1612,13 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       const float p3 = ex2(fmaf(s[mt][3], sl2, -ms1));
       l0 += p0 + p2;
       l1 += p1 + p3;
-      float va = 1.f, vb = 1.f;
-      if constexpr (I8) { va = sc_cur.val(mt * 16, g8) * vinv; vb = sc_cur.val(mt * 16 + 8, g8) * vinv; }
-      pb[mt][0] = movmatrix_trans(I8 ? pack2<BF16>(p0 * va, p1 * va) : pack2<BF16>(p0, p1));  // (keys 16mt+2c, +1 ; q g)
-      pb[mt][1] = movmatrix_trans(I8 ? pack2<BF16>(p2 * vb, p3 * vb) : pack2<BF16>(p2, p3));  // (keys 16mt+8+2c, +1 ; q g)
+      if constexpr (I8) {
+        pb[mt][0] = movmatrix_trans(pack2<BF16>(p0 * va[mt], p1 * va[mt]));
+        pb[mt][1] = movmatrix_trans(pack2<BF16>(p2 * vb[mt], p3 * vb[mt]));
+      } else {
+        pb[mt][0] = movmatrix_trans(pack2<BF16>(p0, p1));  // (keys 16mt+2c, +1 ; q g)
+        pb[mt][1] = movmatrix_trans(pack2<BF16>(p2, p3));  // (keys 16mt+8+2c, +1 ; q g)
+      }
     }
 
     // ---- O^T += V^T P^T.  Rows of V past the sequence end may hold anything (NaN bit
@@ -1473,11 +1661,11 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
               x3 = __byte_perm(x3, 0, 0x3120);
             }
             uint32_t a0, a1, a2, a3;
-            widen(x0, a0, a1);  // row g: d = 16ch + 2g ; row g+8: d = 16ch + 2g + 1 (keys lo)
-            widen(x1, a2, a3);  // same rows, keys hi
+            widen_v(x0, a0, a1);  // row g: d = 16ch + 2g ; row g+8: d = 16ch + 2g + 1 (keys lo)
+            widen_v(x1, a2, a3);  // same rows, keys hi
             mma16816r<false>(o[2 * cp], a0, a1, a2, a3, pb[mt][0], pb[mt][1]);
-            widen(x2, a0, a1);
-            widen(x3, a2, a3);
+            widen_v(x2, a0, a1);
+            widen_v(x3, a2, a3);
             mma16816r<false>(o[2 * cp + 1], a0, a1, a2, a3, pb[mt][0], pb[mt][1]);
           }
         }
@@ -1966,7 +2154,8 @@ inline int launch_attn_hd(int nw, const CUtensorMap& tmK, const CUtensorMap& tmV
   }
 }
 
-// int8 pools: the e4m3 geometry of each kernel
+// int8 pools: the e4m3 geometry of each kernel, but 8 warps for the 16-row kernel (with 12 it spills: a 4-token verify of 64
+// sequences U[2k, 16k], 32/8 heads of 128, 361 | 345 us; 48 sequences U[0, 5k], 16/4 heads of 64, 48 | 42 us)
 template <int HD>
 inline int launch_i8_hd(bool decode8, bool rows32, const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnParams& p, int grid,
                         int dev, cudaStream_t stream) {
@@ -1974,8 +2163,8 @@ inline int launch_i8_hd(bool decode8, bool rows32, const CUtensorMap& tmK, const
                               : launch_rows32_variant<1, HD, false, false, true>(tmK, tmV, p, grid, dev, stream);
   if (decode8) return p.gather ? launch_decode_variant<1, HD, false, 12, 2, true, true>(tmK, tmV, p, grid, dev, stream)
                                : launch_decode_variant<1, HD, false, 12, 2, false, true>(tmK, tmV, p, grid, dev, stream);
-  return p.gather ? launch_attn_variant<1, HD, false, 12, 2, true, true>(tmK, tmV, p, grid, dev, stream)
-                  : launch_attn_variant<1, HD, false, 12, 2, false, true>(tmK, tmV, p, grid, dev, stream);
+  return p.gather ? launch_attn_variant<1, HD, false, 8, 2, true, true>(tmK, tmV, p, grid, dev, stream)
+                  : launch_attn_variant<1, HD, false, 8, 2, false, true>(tmK, tmV, p, grid, dev, stream);
 }
 
 template <int KVB, bool BF16>
@@ -2313,6 +2502,7 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
   KB200_REQUIRE(kv_is_8bit(a->kv_dtype) || a->kv_dtype == a->q_dtype, "K/V dtype must equal q dtype or be E4M3 or I8");
   const bool i8 = a->kv_dtype == KB200_DTYPE_I8;
   KB200_REQUIRE(!i8 || (a->k_block_scale && a->v_block_scale), "int8 pools need k_block_scale and v_block_scale");
+  KB200_REQUIRE(!i8 || a->n_pages <= 0x7fffffff, "too many pages");
   KB200_REQUIRE(!i8 || a->block_scale_page_stride >= a->n_kv_heads, "block_scale_page_stride is smaller than n_kv_heads");
   if (a->head_dim != 64 && a->head_dim != 128)
     return fail(KB200_ERR_UNSUPPORTED, "head_dim %d is not supported (64 or 128)", a->head_dim);
@@ -2356,7 +2546,7 @@ inline int launch_attention_pass(const kb200_attn_args* a, int k_skip, int fixed
   // (12 warps x 2 stages; 8 x 3 and 6 x 4 -- more tiles in flight per warp, fewer warps -- measured 2 % and
   // 13 % slower on the short contexts of a shared-prefix batch)
   const bool rows32 = use_rows32_kernel(a);   // (8 warps: two output accumulators per thread need the registers)
-  const int nw = rows32 ? 8 : (kv_is_8bit(a->kv_dtype) || decode8) ? 12 : 8;
+  const int nw = rows32 || (i8 && !decode8) ? 8 : (kv_is_8bit(a->kv_dtype) || decode8) ? 12 : 8;
   const int n_workers = grid * nw;
   const AttnWorkspace wl = attn_workspace_layout(a->batch, a->total_q, a->n_q_heads, hkv, hd, grid * kAttnMaxWarps, rows32);
   const uint64_t ws_need = attn_pass_workspace_need(a, sms);

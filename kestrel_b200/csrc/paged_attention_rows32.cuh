@@ -107,6 +107,8 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   bool valid[2][2];
   float sl2 = 0.f, lazy = 0.f, vscale = 1.f;
   [[maybe_unused]] float vref = 0.f, vinv = 0.f;   // (I8) largest V scale seen, and what a V scale is multiplied by
+  [[maybe_unused]] float row_init = 0.f;                   // (I8) what the scores of row `lane` of the segment start with
+  [[maybe_unused]] const bool uni16 = p.page_size >= 16;   // (I8) 16 neighbouring keys share their scales
   int h = 0;
   bool two = false;            // the second block has rows at all (warp-uniform)
   bool fresh = true;
@@ -171,7 +173,16 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             v.z = pack2<false>(bf16_bits_to_float(v.z & 0xffffu), bf16_bits_to_float(v.z >> 16));
             v.w = pack2<false>(bf16_bits_to_float(v.w & 0xffffu), bf16_bits_to_float(v.w >> 16));
           }
-          if constexpr (I8) { pair_02_13(v.x, v.y); pair_02_13(v.z, v.w); }   // (4c + {0, 2} and 4c + {1, 3} there)
+          if constexpr (I8) {
+            float rs = (f16x2_sum(v.x) + f16x2_sum(v.y)) + (f16x2_sum(v.z) + f16x2_sum(v.w));   // the row's sum, for its lane
+#pragma unroll
+            for (int d = 1; d < QCH; d <<= 1) rs += __shfl_xor_sync(0xffffffffu, rs, d);
+            constexpr int RPI = 32 / QCH;   // rows of one round: lane RPI * i + j takes the sum of the j-th
+            rs = __shfl_sync(0xffffffffu, rs, (lane % RPI) * QCH);
+            if (lane / RPI == i) row_init = rs * kI8KeyOffset;
+            pair_02_13(v.x, v.y);   // (4c + {0, 2} and 4c + {1, 3} there)
+            pair_02_13(v.z, v.w);
+          }
           const int grp = gc >> 1, byte = 8 * (gc & 1);
           const int ca = 2 * grp, cb = 2 * grp + 1;
           *reinterpret_cast<uint2*>(row + (((ca & ~7) | ((ca & 7) ^ (r & 7))) << 4) + byte) = make_uint2(v.x, v.z);
@@ -196,7 +207,11 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       return q_lane + q_x[ks & 3] + (uint32_t)(blk * 16 * L::Q_ROW_BYTES + ((2 * ks) & 8) * 16);
     };
 
-    auto widen = [](uint32_t x, uint32_t& e, uint32_t& o_) {
+    auto widen_k = [](uint32_t x, uint32_t& e, uint32_t& o_) {
+      if constexpr (I8) i8x4_to_u16x4(x, e, o_);
+      else e4m3x4_to_f16x4(x, e, o_);
+    };
+    auto widen_v = [](uint32_t x, uint32_t& e, uint32_t& o_) {
       if constexpr (I8) i8x4_to_f16x4(x, e, o_);
       else e4m3x4_to_f16x4(x, e, o_);
     };
@@ -206,6 +221,14 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
       for (int n = 0; n < NT8; ++n) s[blk][n][0] = s[blk][n][1] = s[blk][n][2] = s[blk][n][3] = 0.f;
+    if constexpr (I8) {
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        const float a = __shfl_sync(0xffffffffu, row_init, blk * 16 + g8), b = __shfl_sync(0xffffffffu, row_init, blk * 16 + 8 + g8);
+#pragma unroll
+        for (int n = 0; n < NT8; ++n) { s[blk][n][0] = s[blk][n][1] = a; s[blk][n][2] = s[blk][n][3] = b; }
+      }
+    }
     if constexpr (KVB == 2) {
 #pragma unroll
       for (int q4 = 0; q4 < HD / 32; ++q4) {
@@ -247,12 +270,12 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             uint32_t x0, x1;
             ldsm_x2(x0, x1, addr);
             uint32_t b0, b1;
-            widen(x0, b0, b1);
+            widen_k(x0, b0, b1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(s[blk][n], qa[blk][0], b0, b1);
             }
-            widen(x1, b0, b1);
+            widen_k(x1, b0, b1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(s[blk][n], qa[blk][1], b0, b1);
@@ -268,12 +291,24 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     const bool need_mask = key_last > min_lim || (p.window_left >= 0 && key0 < cc.L - 1 - p.window_left);
     uint32_t pf[2][NKS][4];
     if constexpr (I8) {
+      sc_cur.apply_unit(kI8KeyUnit);
+      if (uni16) {
 #pragma unroll
-      for (int n = 0; n < NT8; ++n) {
-        const float ka = sc_cur.key(n * 8, 2 * c4), kb = sc_cur.key(n * 8, 2 * c4 + 1);
+        for (int n = 0; n < NT8; n += 2) {
+          const float ka = sc_cur.key(n * 8, 0);
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk) {
-          s[blk][n][0] *= ka; s[blk][n][1] *= kb; s[blk][n][2] *= ka; s[blk][n][3] *= kb;
+          for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { s[blk][n][i] *= ka; s[blk][n + 1][i] *= ka; }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT8; ++n) {
+          const float ka = sc_cur.key(n * 8, 2 * c4), kb = sc_cur.key(n * 8, 2 * c4 + 1);
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+            s[blk][n][0] *= ka; s[blk][n][1] *= kb; s[blk][n][2] *= ka; s[blk][n][3] *= kb;
+          }
         }
       }
       const float vmax = sc_cur.max_val();
@@ -287,7 +322,7 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           }
         vref = vmax;
         vinv = kVScaleUpLazy / vmax;
-        vscale = vmax * (1.f / kVScaleUpLazy);
+        vscale = vmax * (kI8ValUnit / kVScaleUpLazy);
       }
     }
 #pragma unroll
@@ -333,6 +368,7 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       }
       const float ms0 = (m0 == -INFINITY) ? 0.f : m0 * sl2;
       const float ms1 = (m1 == -INFINITY) ? 0.f : m1 * sl2;
+      [[maybe_unused]] float va = 0.f, vb = 0.f;
 #pragma unroll
       for (int n = 0; n < NT8; ++n) {
         const float p0 = ex2(fmaf(s[blk][n][0], sl2, -ms0));
@@ -342,7 +378,8 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         ls[blk][0] += p0 + p1;
         ls[blk][1] += p2 + p3;
         if constexpr (I8) {
-          const float va = sc_cur.val(n * 8, 2 * c4) * vinv, vb = sc_cur.val(n * 8, 2 * c4 + 1) * vinv;
+          if (!uni16 || n % 2 == 0) va = vb = sc_cur.val(n * 8, uni16 ? 0 : 2 * c4) * vinv;
+          if (!uni16) vb = sc_cur.val(n * 8, 2 * c4 + 1) * vinv;
           pf[blk][n >> 1][(n & 1) * 2 + 0] = pack2<BF16>(p0 * va, p1 * vb);
           pf[blk][n >> 1][(n & 1) * 2 + 1] = pack2<BF16>(p2 * va, p3 * vb);
         } else {
@@ -394,15 +431,15 @@ paged_attn_rows32_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
               x3 = __byte_perm(x3, 0, 0x3120);
             }
             uint32_t e0, o0, e1, o1;
-            widen(x0, e0, o0);
-            widen(x1, e1, o1);
+            widen_v(x0, e0, o0);
+            widen_v(x1, e1, o1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(o[blk][4 * q2 + 0], pf[blk][ks], e0, e1);  // d = 16*(2*q2)   + 2g
               mma16816<false>(o[blk][4 * q2 + 1], pf[blk][ks], o0, o1);  // d = 16*(2*q2)   + 2g + 1
             }
-            widen(x2, e0, o0);
-            widen(x3, e1, o1);
+            widen_v(x2, e0, o0);
+            widen_v(x3, e1, o1);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
               mma16816<false>(o[blk][4 * q2 + 2], pf[blk][ks], e0, e1);  // d = 16*(2*q2+1) + 2g

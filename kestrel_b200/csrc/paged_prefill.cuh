@@ -216,17 +216,29 @@ __host__ __device__ constexpr uint32_t umma_idesc(bool bf16, bool b_mn_major, in
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPfTileRows >> 4) << 24);
 }
 
-// Four int8 codes -> (code + 1/2) * s in the operand type.  A byte, its sign flipped, dropped into bits 8-15 of 2^15 is
-// 2^15 + 128 + code in fp32; one fma by s and off = -(2^15 + 127.5) s does the rest exactly (s a power of two).
+// Four int8 codes -> (code + 1/2) s in the operand type, exactly (s a power of two): a byte with its sign flipped, u = code + 128,
+// in the low half of 16 bits is the subnormal number u 2^-24 (f16) or u 2^-133 (bf16); one fma makes (code + 1/2) 2^-9 or 2^-6
+// of it, a product by su = s 2^9 or s 2^6 the rest (f16: s and 2^9 one after the other, their product may pass 65504).
 template <bool BF16>
-__device__ __forceinline__ void i8x4_scaled(uint32_t x, float s, float off, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ uint32_t i8_scale2(uint32_t u2, uint32_t su) {
+  uint32_t r;
+  if constexpr (BF16) {
+    // 0x7f00: 2^127; 0xbfff: -255 / 128
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u2), "r"(0x7f007f00u), "r"(0xbfffbfffu));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(su));
+  } else {
+    // 0x7800: 2^15; 0xb3f8: -255 / 1024; 0x6000: 2^9
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u2), "r"(0x78007800u), "r"(0xb3f8b3f8u));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0x60006000u));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(su));
+  }
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void i8x4_scaled(uint32_t x, uint32_t su, uint32_t& lo, uint32_t& hi) {
   x ^= 0x80808080u;
-  const float a = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7604)), s, off);
-  const float b = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7614)), s, off);
-  const float c = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7624)), s, off);
-  const float d = fmaf(__uint_as_float(__byte_perm(x, 0x47000000u, 0x7634)), s, off);
-  lo = pack2<BF16>(a, b);
-  hi = pack2<BF16>(c, d);
+  lo = i8_scale2<BF16>(__byte_perm(x, 0u, 0x4140), su);
+  hi = i8_scale2<BF16>(__byte_perm(x, 0u, 0x4342), su);
 }
 
 // BF16: dtype of q and out.  KV8: K/V pools hold e4m3 codes; the tiles are widened to f16 in shared memory
@@ -456,16 +468,20 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       }
       const uint8_t* src = sgen + SM::OFF_STG + s8 * SM::STG_TILE + r * RB8;
       uint8_t* dst = sgen + RING_OFF + c * SM::KV_TILE + r * 128;
+      [[maybe_unused]] uint32_t su = 0;
+      if constexpr (I8) {
+        const float s = ((idx & 1) ? sv : sk) * (MMA_BF16 ? 64.f : 1.f);
+        su = pack2<MMA_BF16>(s, s);
+      }
 #pragma unroll
       for (int ch = 0; ch < RB8 / 16; ++ch) {
         const uint4 x = *reinterpret_cast<const uint4*>(src + ((ch ^ (int)swz<RB8>(r)) << 4));
         uint4 lo4, hi4;   // elements 16ch .. 16ch+7 and 16ch+8 .. 16ch+15 as f16 (I8: in q's type)
         if constexpr (I8) {
-          const float s = (idx & 1) ? sv : sk, off = -32895.5f * s;
-          i8x4_scaled<MMA_BF16>(x.x, s, off, lo4.x, lo4.y);
-          i8x4_scaled<MMA_BF16>(x.y, s, off, lo4.z, lo4.w);
-          i8x4_scaled<MMA_BF16>(x.z, s, off, hi4.x, hi4.y);
-          i8x4_scaled<MMA_BF16>(x.w, s, off, hi4.z, hi4.w);
+          i8x4_scaled<MMA_BF16>(x.x, su, lo4.x, lo4.y);
+          i8x4_scaled<MMA_BF16>(x.y, su, lo4.z, lo4.w);
+          i8x4_scaled<MMA_BF16>(x.z, su, hi4.x, hi4.y);
+          i8x4_scaled<MMA_BF16>(x.w, su, hi4.z, hi4.w);
         } else {
           e4m3x4_to_f16x4(x.x, lo4.x, lo4.y);
           e4m3x4_to_f16x4(x.y, lo4.z, lo4.w);

@@ -49,8 +49,8 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 def attention(q, k_codes, k_scales, v_codes, v_scales, page_table, seqused_k, *, scale, causal=True, window=None,
               rows=None, visible_until=None):
     """float64 paged attention.  ``q [B, Sq, Hq, D]``; ``rows[b]``: valid query rows.  Returns ``(out, lse, weight,
-    score)``: the output and log-sum-exp, and per output element ``sum_j p_j |v_j|`` and the largest ``scale *
-    sum_d |q_d k_d|`` of its row, which is what rounding errors are proportional to.  Rows without a key: zeros and -inf."""
+    score, reach)``: the output and log-sum-exp, and what rounding errors are proportional to: per output element ``sum_j p_j
+    |v_j|``, per row the largest ``scale * sum_d |q_d k_d|`` and the largest ``scale * max|q| * sum_d |k_d|``.  Rows without a key: zeros and -inf."""
     B, Sq, Hq, D = q.shape
     Hkv, P = k_codes.shape[1], k_codes.shape[2]
     g = Hq // Hkv
@@ -59,6 +59,7 @@ def attention(q, k_codes, k_scales, v_codes, v_scales, page_table, seqused_k, *,
     weight = torch.zeros_like(out)
     lse = torch.full((B, Hq, Sq), -math.inf, dtype=torch.float64, device=dev)
     score = torch.zeros(B, Sq, Hq, 1, dtype=torch.float64, device=dev)
+    reach = torch.zeros_like(score)
     for b in range(B):
         n = int(seqused_k[b])
         sq = Sq if rows is None else int(rows[b])
@@ -83,5 +84,7 @@ def attention(q, k_codes, k_scales, v_codes, v_scales, page_table, seqused_k, *,
         out[b, :sq] = torch.einsum("hjn,nhd->jhd", p, V)
         weight[b, :sq] = torch.einsum("hjn,nhd->jhd", p, V.abs())
         lse[b, :, :sq] = torch.logsumexp(z, -1)
+        ka = (K.abs().sum(-1).transpose(0, 1).unsqueeze(1) * scale).expand(Hq, sq, n).masked_fill(~ok, 0.0).amax(-1)
+        reach[b, :sq] = (ka.transpose(0, 1) * x.abs().amax(-1)).unsqueeze(-1)
         score[b, :sq] = za.masked_fill(~ok, 0.0).amax(-1).transpose(0, 1).unsqueeze(-1)
-    return out, lse, weight, score
+    return out, lse, weight, score, reach

@@ -7,6 +7,8 @@ Attention: the pool's values are exact in both computations, so an output elemen
   u_p A                                       the rounding of the softmax weights, A = sum_j p_j |v_j|
   A (4 D 2^-24 S + 2^-20 + 2 n 2^-24)         fp32 products of D terms (S = scale * sum |q k| of the row, twice for an accumulator
                                               that truncates, numerator and denominator), the exponential, sums of n terms
+  A 2 R 2^-15.9                               up to 16 packed rows the query is a 16-bit number relative to its row's largest, off by
+                                              max|q| / 65024 at most: R = scale * max|q| * sum |k| of the row's worst key
   n 2^-25 max|v|                              weights below f16's normal range
 with u_p = 2^-8 where the products run on bf16 operands (prompt chunks of bf16 queries) and 2^-11 elsewhere.
 """
@@ -280,12 +282,13 @@ def _half_step(dtype):
 
 
 def _check(got, p, *, lse=None, bf16_products=False, **kw):
-    out, want_lse, weight, score = O.attention(p["q"], p["kc"], p["ks"], p["vc"], p["vs"], p["table"], p["lens"], scale=p["scale"], **kw)
+    out, want_lse, weight, score, reach = O.attention(p["q"], p["kc"], p["ks"], p["vc"], p["vs"], p["table"], p["lens"], scale=p["scale"], **kw)
     D = p["q"].shape[-1]
     n = int(p["lens"].max())
     vmax = float((128 * p["vs"].max()).double())
     u_p = _half_step(torch.bfloat16) if bf16_products and p["q"].dtype == torch.bfloat16 else _half_step(torch.float16)
-    rel = u_p + 4 * D * 2.0 ** -24 * score + 2.0 ** -20 + 2 * n * 2.0 ** -24
+    reach = reach / 65024 * 2
+    rel = u_p + 4 * D * 2.0 ** -24 * score + reach + 2.0 ** -20 + 2 * n * 2.0 ** -24
     tol = weight * rel + n * 2.0 ** -25 * vmax
     tol = tol + _half_step(p["q"].dtype) * (out.abs() + tol) + 1e-30
     err = (got.double() - out).abs()
@@ -296,7 +299,7 @@ def _check(got, p, *, lse=None, bf16_products=False, **kw):
         assert bool(same.all())
         d = (lse.double() - want_lse).abs()[torch.isfinite(want_lse)]
         # fp32 scores and sum: the same relative terms as the weights', and the value's own rounding
-        most = 4 * D * 2.0 ** -24 * float(score.max()) + 2.0 ** -19 + 2 * n * 2.0 ** -24 + 2.0 ** -22 * float(want_lse[torch.isfinite(want_lse)].abs().max())
+        most = 4 * D * 2.0 ** -24 * float(score.max()) + float(reach.max()) + 2.0 ** -19 + 2 * n * 2.0 ** -24 + 2.0 ** -22 * float(want_lse[torch.isfinite(want_lse)].abs().max())
         assert float(d.max()) <= most
 
 
@@ -401,7 +404,7 @@ def test_shared_prefix(Sq):
     out, _ = _run(p, causal=True, shared_prefix_pages=10)
     plain, _ = _run(p, causal=True)
     # three roundings to bf16 (two partials and the sum) and bf16 weights in the prefix pass, on values up to A
-    _, _, weight, _ = O.attention(p["q"], p["kc"], p["ks"], p["vc"], p["vs"], p["table"], p["lens"], scale=p["scale"])
+    _, _, weight, _, _ = O.attention(p["q"], p["kc"], p["ks"], p["vc"], p["vs"], p["table"], p["lens"], scale=p["scale"])
     assert bool(((out.double() - plain.double()).abs() <= 5 * 2.0 ** -8 * weight + 1e-6).all())
 
 
