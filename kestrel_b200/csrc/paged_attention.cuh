@@ -321,10 +321,15 @@ __device__ __forceinline__ void q4_to_floats(uint32_t w0, uint32_t w1, bool bf16
     f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
   }
 }
+__device__ __forceinline__ float max_nan(float a, float b) {   // (a NaN stays: the row's scores are NaN, as on other pools)
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float q4_max(uint32_t w0, uint32_t w1, bool bf16) {
   float f[4];
   q4_to_floats(w0, w1, bf16, f);
-  return fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+  return max_nan(max_nan(fabsf(f[0]), fabsf(f[1])), max_nan(fabsf(f[2]), fabsf(f[3])));
 }
 // the high and low bytes of n = rint(q inv), four to a word; returns their sum
 __device__ __forceinline__ int q4_to_bytes(uint32_t w0, uint32_t w1, bool bf16, float inv, uint32_t& hi, uint32_t& lo) {
@@ -860,13 +865,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           float t0 = 0.f, t1 = 0.f;
 #pragma unroll
           for (int ch = 0; ch < NQF; ++ch) {
-            t0 = fmaxf(t0, q4_max(qf[ch][0], qf[ch][2], qbf));
-            t1 = fmaxf(t1, q4_max(qf[ch][1], qf[ch][3], qbf));
+            t0 = max_nan(t0, q4_max(qf[ch][0], qf[ch][2], qbf));
+            t1 = max_nan(t1, q4_max(qf[ch][1], qf[ch][3], qbf));
           }
 #pragma unroll
           for (int d = 1; d < 4; d <<= 1) {
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+            t0 = max_nan(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+            t1 = max_nan(t1, __shfl_xor_sync(0xffffffffu, t1, d));
           }
           const float v0 = t0 > 0.f ? kI8QueryMax / t0 : 0.f, v1 = t1 > 0.f ? kI8QueryMax / t1 : 0.f;
           int n0 = 0, n1 = 0;
@@ -1404,9 +1409,9 @@ paged_attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           const bool qbf = p.q_is_bf16 != 0;
           float top = 0.f;
 #pragma unroll
-          for (int ch = 0; ch < NDT; ++ch) top = fmaxf(top, q4_max(qb[ch][0], qb[ch][1], qbf));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          for (int ch = 0; ch < NDT; ++ch) top = max_nan(top, q4_max(qb[ch][0], qb[ch][1], qbf));
+          top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const float inv = top > 0.f ? kI8QueryMax / top : 0.f;
           int ns = 0;
 #pragma unroll

@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import sys
+from operator import attrgetter
 from typing import Any, NamedTuple, Optional, Sequence
 
 import torch
@@ -594,6 +595,20 @@ def copy_pages(caches: Sequence[torch.Tensor], src_pages, dst_pages) -> None:
                                        src_t.data_ptr(), dst_t.data_ptr(), src_t.numel(), dev, _stream(dev)))
 
 
+_shape_of, _dtype_of = attrgetter("shape"), attrgetter("dtype")
+
+
+def _alike(tensors: Sequence[torch.Tensor], name: str, dev: int) -> bool:
+    """All on GPU ``dev`` (raises otherwise) and of one shape, dtype and strides.  Written for a few dozen pools per call, whose
+    checks are most of what the call costs the host: no Python-level loop unless something is wrong."""
+    if set(map(torch.Tensor.get_device, tensors)) != {dev}:
+        for i, t in enumerate(tensors):
+            if _require_cuda(f"{name}[{i}]", t) != dev:
+                raise ValueError(f"{name}[{i}] lives on a different device than the tables")
+    same_strides = all(map(torch.Tensor.is_contiguous, tensors)) or len(set(map(torch.Tensor.stride, tensors))) == 1
+    return same_strides and len(set(map(_shape_of, tensors))) == 1 and len(set(map(_dtype_of, tensors))) == 1
+
+
 def reorder_beam_pages(beam_table: torch.Tensor, own_table: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor,
                        page_size: int, caches: Sequence[torch.Tensor], *, scales: Optional[Sequence[torch.Tensor]] = None,
                        own_rows: Optional[torch.Tensor] = None) -> None:
@@ -636,23 +651,21 @@ def reorder_beam_pages(beam_table: torch.Tensor, own_table: torch.Tensor, parent
         stride = first.stride()
         if stride[3] != 1 or stride[2] != shape[3]:
             raise ValueError("the tokens of one page and head must be contiguous")
-        dense = first.is_contiguous()
-        for i, c in enumerate(caches):   # (a few dozen pools: the checks are most of what the call costs the host)
-            if c.shape != shape or c.dtype != dtype or not (dense and c.is_contiguous() or c.stride() == stride):
-                raise ValueError("all pools must share shape, strides and dtype")
-            if _require_cuda("caches[i]", c) != dev:
-                raise ValueError("all pools must live on the tables' device")
+        if not _alike(caches, "caches", dev):
+            raise ValueError("all pools must share shape, strides and dtype")
         n_pages, H, row_bytes = shape[0], shape[1], shape[3] * es
         page_stride, head_stride = stride[0] * es, stride[1] * es
     n_scales = len(scales) if scales is not None else 0
     if n_scales:
-        want, s_stride = torch.Size((n_pages, H)), scales[0].stride()
-        for s in scales:
-            if s.shape != want or s.dtype != torch.float32 or s.stride() != s_stride or _require_cuda("scales[i]", s) != dev or s_stride[1] != 1:
-                raise ValueError("scales must be fp32 [n_pages, n_heads] arrays with equal strides on the tables' device")
-        scale_stride = s_stride[0]
-    ptrs = (C.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
-    sptrs = (C.c_void_p * max(1, n_scales))(*[s.data_ptr() for s in scales or ()])
+        s0 = scales[0]
+        if not _alike(scales, "scales", dev) or s0.shape != (n_pages, H) or s0.dtype != torch.float32 or s0.stride(1) != 1:
+            raise ValueError("scales must be fp32 [n_pages, n_heads] arrays with equal strides on the tables' device")
+        scale_stride = s0.stride(0)
+    at = [*map(torch.Tensor.data_ptr, caches), *map(torch.Tensor.data_ptr, scales or ())]
+    if len(set(at)) != len(at):   # (it would be permuted twice)
+        raise ValueError("a pool or scale array is listed twice")
+    ptrs = (C.c_void_p * max(1, len(caches)))(*at[:len(caches)])
+    sptrs = (C.c_void_p * max(1, n_scales))(*at[len(caches):])
     if B == 0 or W == 0:
         return
     _native.check(_native.load().kb200_reorder_beam_pages(

@@ -235,6 +235,7 @@ def test_reorder_refusals():
     kernels.reorder_beam_pages(**ok)
     for bad, err in ((dict(own_table=t), ValueError), (dict(beam_table=t[:1]), ValueError), (dict(parents=p[0]), ValueError), (dict(lengths=L.long()), ValueError),
                      (dict(page_size=8), ValueError), (dict(caches=[c[0], c[1].half()]), ValueError), (dict(caches=[c[0].cpu()]), RuntimeError),
+                     (dict(caches=[c[0], c[1], c[0]]), ValueError),
                      (dict(scales=[torch.zeros(3, 1, device=DEV)]), ValueError), (dict(own_rows=p), ValueError)):
         with pytest.raises(err):
             kernels.reorder_beam_pages(**{**ok, **bad})

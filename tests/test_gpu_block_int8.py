@@ -9,6 +9,7 @@ Attention: the pool's values are exact in both computations, so an output elemen
                                               that truncates, numerator and denominator), the exponential, sums of n terms
   A 2 R 2^-15.9                               up to 16 packed rows the query is a 16-bit number relative to its row's largest, off by
                                               max|q| / 65024 at most: R = scale * max|q| * sum |k| of the row's worst key
+  A 4 D 2^-24 scale 128 k_scale sum |q|       17 to 64 packed rows: K enters the products as code + 128, an offset taken out again
   n 2^-25 max|v|                              weights below f16's normal range
 with u_p = 2^-8 where the products run on bf16 operands (prompt chunks of bf16 queries) and 2^-11 elsewhere.
 """
@@ -288,6 +289,8 @@ def _check(got, p, *, lse=None, bf16_products=False, **kw):
     vmax = float((128 * p["vs"].max()).double())
     u_p = _half_step(torch.bfloat16) if bf16_products and p["q"].dtype == torch.bfloat16 else _half_step(torch.float16)
     reach = reach / 65024 * 2
+    offset = 4 * D * 2.0 ** -24 * p["scale"] * 128 * float(p["ks"].max()) * p["q"].double().abs().sum(-1, keepdim=True)
+    reach = reach + offset
     rel = u_p + 4 * D * 2.0 ** -24 * score + reach + 2.0 ** -20 + 2 * n * 2.0 ** -24
     tol = weight * rel + n * 2.0 ** -25 * vmax
     tol = tol + _half_step(p["q"].dtype) * (out.abs() + tol) + 1e-30
