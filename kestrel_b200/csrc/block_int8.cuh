@@ -9,9 +9,14 @@
 //
 // Work.  HBM-bound: T * H * D * 2 * (in + 1) bytes.  The tokens of one block form a *run* of the slot mapping (the page stays
 // the same); a run's first token decides who handles it, so a block has one owner per call and nothing is atomic.
-// A CTA looks after `window` tokens of one head of K or V: runs of up to 16 tokens that start there go to one warp each, longer
-// ones to all of its warps together.  A run's rows are asked for together with the block's old scale and stay in registers
-// between the maximum and the codes (rows that do not fit are read again, out of L1).
+//   append_block_int8_kernel        few tokens (a decode step, a short chunk): a CTA looks after `window` tokens of one head of K or V,
+//                                   runs of up to 16 tokens that start there go to one warp each, longer ones to all of its warps
+//                                   together; rows are asked for together with the block's old scale and stay in registers
+//                                   between the maximum and the codes
+//   append_block_int8_warps_kernel  many tokens: every warp has a window of its own
+// Measured, 8 heads of 128, bf16 rows: 256 single tokens 6.4 us (latency: slots, then rows and scale, then codes); eight
+// chunks of 1500 to 2600 tokens 34 us = 3.1 TB/s with a warp per window, 58 us with a CTA per window.  What is left: the
+// second pass comes out of L2, and a run's passes wait for each other.
 #pragma once
 
 #include <type_traits>
