@@ -1032,7 +1032,8 @@ def beam_step_from_logits(logits: torch.Tensor, scores: torch.Tensor, n_out: int
     ``logits`` ``[B * W, V]`` fp32 / fp16 / bf16 (a NaN counts as -inf); ``scores`` fp32 ``[B, W]``, finite or -inf (a
     beam that does not exist yet); ``finished`` bool ``[B, W]``: such a beam has one continuation, ``end_token``, at its own
     score.  ``n_out`` at most 64, usually ``W`` or ``2 W``.  Returns tokens, parent beams and scores, all ``[B, n_out]``
-    (``out``: written there).  Rows with nothing finite offer only candidates of -inf.
+    (``out``: written there).  Rows with nothing finite offer only candidates of -inf.  The scratch memory belongs to the
+    stream of the call or capture, as :func:`flash_attn_fwd`'s: graphs captured on one stream are replayed one after another.
     """
     dev = _require_cuda("logits", logits)
     if logits.ndim != 2 or logits.stride(1) != 1:
