@@ -733,7 +733,7 @@ struct TileProducer {
 // I8: K/V are int8 codes with a scale per (page, head): scores are multiplied by the key's K scale, weights by its V scale.
 // Measured, 32/8 heads of 128 in pages of 16, one call (e4m3 pool of the same shape): 64 sequences U[2k, 16k] 248 us = 5.4 TB/s
 // (238), 256 of them 923 us = 5.2 TB/s (778); a 4-token verify of the 64 345 us (244).  What the int8 calls pay over e4m3 is
-// ALU work: V's bytes take a mask, a shift and an fma where e4m3 has a conversion, and every tile its scales.
+// instructions, a third more of them (fmas mostly: V's, the joining of the query's byte planes, the scales of every tile).
 // ---------------------------------------------------------------------------
 template <int KVB, int HD, bool BF16, int NW, int NS, bool GATHER, bool I8 = false>
 __global__ void __launch_bounds__(NW * 32, 1)
